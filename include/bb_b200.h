@@ -293,6 +293,93 @@ BB_API int bb_embed_gather(const void* table, int64_t vocab, int64_t row_bytes, 
 BB_API int bb_rmsnorm(void* x, int64_t sx, const void* residual, int64_t sr, const void* weight, void* y, int64_t sy,
                       int64_t rows, int64_t cols, float eps, int dtype, bb_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Quantised KV cache: keys and values of one layer in 4- or 8-bit codes, decoded from directly.
+ *
+ * Format. A row (one token of one KV head) holds d codes of `bits` bits; every `group` consecutive
+ * dimensions share a step and a low value (bf16 each), and code c stands for low + step * c.
+ * Written: low = bf16 rounded down of the group's minimum; step = bf16 rounded up of
+ * (maximum - low) / (2^bits - 1); code = (x - low) / step rounded to nearest even; a step below
+ * 2^-100 is stored as 0 (the group reads back as `low`), and a group whose range is not finite (a
+ * NaN, an infinity, an fp32 overflow) as NaN step and low (it reads back as NaN).
+ * Order: with G = d / 32, the code of dimension 32 g + run a + i (0 <= i < run) stands at place
+ * (a G + g) run + i of its row, run = 8 for keys and 4 for values: the order in which the attention
+ * kernel's matrix fragments take them. 4-bit rows keep place 2b in the low half of byte b and
+ * place 2b + 1 in its high half; 8-bit rows keep place b in byte b.
+ * Buffers: codes [Hkv, cap, d * bits / 8] bytes, meta [Hkv, cap, d / group, 2] bf16 as (step, low);
+ * rows dense, heads at any stride of whole rows; all bases on 16-byte boundaries, code heads on
+ * 16-byte multiples. d a multiple of 32 up to 128; group 32, 64, 96 or 128 dividing d.
+ */
+typedef struct {
+  void* k_codes; void* k_meta;
+  void* v_codes; void* v_meta;
+  int64_t k_codes_h, k_meta_h, v_codes_h, v_meta_h; /* head strides: codes in bytes, meta in (step, low) pairs */
+  int64_t kv_heads, cap, d;
+  int bits;  /* 4 or 8 */
+  int group;
+} bb_qkv_cache;
+
+/* bb_qkv_write: rows k, v [Hkv, t, d] (fp16, bf16 or fp32; rows on 16-byte boundaries) into the cache
+ * at positions at, at + 1, ... (at = *at_dev when at_dev != NULL); positions outside [0, cap) are
+ * skipped. out_k / out_v (both or neither): the values that the written codes stand for, in the
+ * input dtype, [Hkv, t, d] (also for skipped rows).
+ *
+ * bb_qkv_read: the values of rows start, start + 1, ... start + rows - 1, or of rows positions[Hkv, rows]
+ * (int32, or int64 with pos_i64), as [Hkv, rows, d] in `dtype`; positions outside [0, cap) give zeros. */
+typedef struct {
+  bb_qkv_cache cache;
+  const void* k; int64_t sk_h, sk_t;
+  const void* v; int64_t sv_h, sv_t;
+  int64_t t, at; const int64_t* at_dev;
+  void* out_k; int64_t sok_h, sok_t;
+  void* out_v; int64_t sov_h, sov_t;
+  int dtype;
+} bb_qkv_write_args;
+
+typedef struct {
+  bb_qkv_cache cache;
+  const void* positions; int64_t sp_h;  /* NULL: the range from `start` */
+  int64_t rows, start;
+  void* out_k; int64_t sok_h, sok_t;
+  void* out_v; int64_t sov_h, sov_t;
+  int dtype;
+  int pos_i64;
+} bb_qkv_read_args;
+
+BB_API int bb_qkv_write(const bb_qkv_write_args* a, bb_stream_t stream);
+BB_API int bb_qkv_read(const bb_qkv_read_args* a, bb_stream_t stream);
+
+/* bb_qkv_decode: attention of the newest t tokens over the quantised cache (the new rows written
+ * first). With n keys cached, token i (0 <= i < t) stands at position p = n - t + i and attends to the
+ * keys of [0, front), of [p - window + 1, p] and of its list idx, none beyond p and none twice
+ * (listed positions outside [front, p - window] are skipped; a position listed twice counts twice). A
+ * token that sees no key gives zeros. idx: [Hkv, route_k] shared by a KV head's query heads, or
+ * [H, route_k]. n = *n_dev (clamped to [0, cap]) when n_dev != NULL.
+ *
+ * bb_qkv_route: for one token q [H, 1, d], the softmax probability of each of the first n keys, averaged
+ * over the query heads of a KV head, -1 outside [front, n - window): out_probs [Hkv, cap] fp32 (may
+ * be NULL); out_idx (may be NULL): [Hkv, route_k] the most probable positions, ascending. */
+typedef struct {
+  bb_qkv_cache cache;
+  const void* q; int64_t sq_h, sq_t;      /* [H, t, d], innermost stride 1 */
+  const void* idx; int64_t si_r;          /* int32, or int64 with idx_i64 */
+  int64_t route_rows, route_k;            /* bb_qkv_route: route_k = keys to select */
+  int64_t n; const int64_t* n_dev;
+  int64_t heads, t, front, window;
+  void* out; int64_t so_h, so_t;          /* [H, t, d] in the q dtype */
+  float* out_probs;
+  void* out_idx; int64_t so_i;
+  int64_t splits;                         /* 0: chosen to fill the GPU */
+  float scale;
+  int dtype;                              /* of q and out: BB_F16 / BB_BF16 */
+  int idx_i64, out_idx_i64;
+} bb_qkv_attn_args;
+
+BB_API int bb_qkv_decode_workspace_size(const bb_qkv_attn_args* a, size_t* bytes);
+BB_API int bb_qkv_decode(const bb_qkv_attn_args* a, void* workspace, size_t workspace_bytes, bb_stream_t stream);
+BB_API int bb_qkv_route_workspace_size(const bb_qkv_attn_args* a, size_t* bytes);
+BB_API int bb_qkv_route(const bb_qkv_attn_args* a, void* workspace, size_t workspace_bytes, bb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

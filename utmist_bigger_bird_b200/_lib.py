@@ -93,6 +93,45 @@ class DecodeArgs(C.Structure):
                 ("dtype", C.c_int), ("idx_i64", C.c_int), ("out_idx_i64", C.c_int)]
 
 
+class QkvCache(C.Structure):
+    _fields_ = [("k_codes", vp), ("k_meta", vp), ("v_codes", vp), ("v_meta", vp),
+                ("k_codes_h", i64), ("k_meta_h", i64), ("v_codes_h", i64), ("v_meta_h", i64),
+                ("kv_heads", i64), ("cap", i64), ("d", i64), ("bits", C.c_int), ("group", C.c_int)]
+
+
+class QkvWriteArgs(C.Structure):
+    _fields_ = [("cache", QkvCache),
+                ("k", vp), ("sk_h", i64), ("sk_t", i64),
+                ("v", vp), ("sv_h", i64), ("sv_t", i64),
+                ("t", i64), ("at", i64), ("at_dev", vp),
+                ("out_k", vp), ("sok_h", i64), ("sok_t", i64),
+                ("out_v", vp), ("sov_h", i64), ("sov_t", i64),
+                ("dtype", C.c_int)]
+
+
+class QkvReadArgs(C.Structure):
+    _fields_ = [("cache", QkvCache),
+                ("positions", vp), ("sp_h", i64),
+                ("rows", i64), ("start", i64),
+                ("out_k", vp), ("sok_h", i64), ("sok_t", i64),
+                ("out_v", vp), ("sov_h", i64), ("sov_t", i64),
+                ("dtype", C.c_int), ("pos_i64", C.c_int)]
+
+
+class QkvAttnArgs(C.Structure):
+    _fields_ = [("cache", QkvCache),
+                ("q", vp), ("sq_h", i64), ("sq_t", i64),
+                ("idx", vp), ("si_r", i64),
+                ("route_rows", i64), ("route_k", i64),
+                ("n", i64), ("n_dev", vp),
+                ("heads", i64), ("t", i64), ("front", i64), ("window", i64),
+                ("out", vp), ("so_h", i64), ("so_t", i64),
+                ("out_probs", vp),
+                ("out_idx", vp), ("so_i", i64),
+                ("splits", i64),
+                ("scale", f32), ("dtype", C.c_int), ("idx_i64", C.c_int), ("out_idx_i64", C.c_int)]
+
+
 EXPORTS = {
     "bb_last_error": (C.c_char_p, []),
     "bb_abi_version": (C.c_int, []),
@@ -116,6 +155,12 @@ EXPORTS = {
     "bb_decode_route": (C.c_int, [C.POINTER(DecodeArgs), vp, C.c_size_t, vp]),
     "bb_silu_mul": (C.c_int, [vp, i64, vp, i64, i64, i64, C.c_int, vp]),
     "bb_embed_gather": (C.c_int, [vp, i64, i64, vp, i64, vp, vp, vp]),
+    "bb_qkv_write": (C.c_int, [C.POINTER(QkvWriteArgs), vp]),
+    "bb_qkv_read": (C.c_int, [C.POINTER(QkvReadArgs), vp]),
+    "bb_qkv_decode_workspace_size": (C.c_int, [C.POINTER(QkvAttnArgs), C.POINTER(C.c_size_t)]),
+    "bb_qkv_decode": (C.c_int, [C.POINTER(QkvAttnArgs), vp, C.c_size_t, vp]),
+    "bb_qkv_route_workspace_size": (C.c_int, [C.POINTER(QkvAttnArgs), C.POINTER(C.c_size_t)]),
+    "bb_qkv_route": (C.c_int, [C.POINTER(QkvAttnArgs), vp, C.c_size_t, vp]),
     "bb_rmsnorm": (C.c_int, [vp, i64, vp, i64, vp, vp, i64, i64, i64, C.c_float, C.c_int, vp]),
 }
 

@@ -66,6 +66,12 @@ int embed_gather(const void* table, int64_t vocab, int64_t row_bytes, const int6
                  int32_t* bad, cudaStream_t stream);
 int rmsnorm(void* x, int64_t sx, const void* r, int64_t sr, const void* w, void* y, int64_t sy, int64_t rows,
             int64_t cols, float eps, int dtype, cudaStream_t stream);
+int qkv_write(const bb_qkv_write_args* a, cudaStream_t stream);
+int qkv_read(const bb_qkv_read_args* a, cudaStream_t stream);
+int qkv_decode_workspace_size(const bb_qkv_attn_args* a, size_t* bytes);
+int qkv_decode(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_t stream);
+int qkv_route_workspace_size(const bb_qkv_attn_args* a, size_t* bytes);
+int qkv_route(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_t stream);
 
 namespace {
 
@@ -247,6 +253,28 @@ int bb_embed_gather(const void* table, int64_t vocab, int64_t row_bytes, const i
 int bb_rmsnorm(void* x, int64_t sx, const void* residual, int64_t sr, const void* weight, void* y, int64_t sy,
                int64_t rows, int64_t cols, float eps, int dtype, bb_stream_t stream) {
   return bb::rmsnorm(x, sx, residual, sr, weight, y, sy, rows, cols, eps, dtype, bb::as_stream(stream));
+}
+
+int bb_qkv_write(const bb_qkv_write_args* a, bb_stream_t stream) { return bb::qkv_write(a, bb::as_stream(stream)); }
+
+int bb_qkv_read(const bb_qkv_read_args* a, bb_stream_t stream) { return bb::qkv_read(a, bb::as_stream(stream)); }
+
+int bb_qkv_decode_workspace_size(const bb_qkv_attn_args* a, size_t* bytes) {
+  if (!bytes) return bb::fail(BB_ERR_ARG, "qkv_decode: null bytes pointer");
+  return bb::qkv_decode_workspace_size(a, bytes);
+}
+
+int bb_qkv_decode(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, bb_stream_t stream) {
+  return bb::qkv_decode(a, ws, ws_bytes, bb::as_stream(stream));
+}
+
+int bb_qkv_route_workspace_size(const bb_qkv_attn_args* a, size_t* bytes) {
+  if (!bytes) return bb::fail(BB_ERR_ARG, "qkv_route: null bytes pointer");
+  return bb::qkv_route_workspace_size(a, bytes);
+}
+
+int bb_qkv_route(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, bb_stream_t stream) {
+  return bb::qkv_route(a, ws, ws_bytes, bb::as_stream(stream));
 }
 
 int bb_flash_workspace_size(const bb_flash_args* a, size_t* bytes) {

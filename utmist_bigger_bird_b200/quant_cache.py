@@ -1,0 +1,255 @@
+"""A layer's KV cache in 4- or 8-bit codes, and the decode step's operators over it.
+
+A 16-bit cache costs ``4 d`` bytes a token and KV head, all of which a dense decode step and the
+decode routing read; with 4-bit codes and groups of 32 it is ``1.25 d``, with groups of 128
+``1.0625 d``. ``QuantKV`` owns the buffers; ``write`` quantises new rows into them (and can return the
+values that the cache now holds, so that a prefill attends to what later steps will read) and
+``read`` gives rows back. ``quant_decode``, ``quant_pooled_probs`` and ``quant_route`` are
+``bigger_bird_decode``, ``pooled_probs`` and ``bigger_bird_route`` on such a cache, without a 16-bit copy
+of it in between. The format and the arithmetic are described at ``bb_qkv_cache`` in
+``include/bb_b200.h``.
+
+Everything runs on the current stream without synchronising; ``n`` and ``at`` may be 1-element GPU
+integer tensors that the kernels read at run time, so a captured CUDA graph follows a growing cache.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib, _ops
+
+__all__ = ["QuantKV", "quant_decode", "quant_pooled_probs", "quant_route"]
+
+_HALF = (torch.float16, torch.bfloat16)
+
+
+class QuantKV:
+    """Codes and (step, low) pairs of ``kv_heads`` x ``capacity`` rows of keys and of values.
+
+    ``bits``: 4 or 8. ``group``: dimensions that share a step and a low value (32, 64, 96 or 128, dividing
+    ``head_dim``, which is a multiple of 32 up to 128). Buffers start at zero, which reads as 0."""
+
+    def __init__(self, kv_heads, capacity, head_dim, *, bits=4, group=32, device="cuda"):
+        if bits not in (4, 8):
+            raise ValueError("QuantKV: bits must be 4 or 8")
+        if head_dim <= 0 or head_dim > 128 or head_dim % 32:
+            raise ValueError("QuantKV: head_dim must be a multiple of 32 up to 128")
+        if group <= 0 or group % 32 or head_dim % group:
+            raise ValueError("QuantKV: group must be a multiple of 32 that divides head_dim")
+        if kv_heads <= 0 or capacity <= 0:
+            raise ValueError("QuantKV: kv_heads and capacity must be positive")
+        codes = [torch.zeros(kv_heads, capacity, head_dim * bits // 8, dtype=torch.uint8, device=device) for _ in "kv"]
+        meta = [torch.zeros(kv_heads, capacity, head_dim // group, 2, dtype=torch.bfloat16, device=device) for _ in "kv"]
+        self._adopt(codes[0], meta[0], codes[1], meta[1], bits)
+
+    @classmethod
+    def from_buffers(cls, k_codes, k_meta, v_codes, v_meta, *, bits):
+        """A cache over the caller's buffers: codes uint8 [Hkv, cap, d * bits / 8], meta bf16
+        [Hkv, cap, d / group, 2] as (step, low); rows dense, heads at any stride."""
+        self = cls.__new__(cls)
+        if bits not in (4, 8):
+            raise ValueError("QuantKV: bits must be 4 or 8")
+        for codes, meta in ((k_codes, k_meta), (v_codes, v_meta)):
+            if codes.dtype != torch.uint8 or meta.dtype != torch.bfloat16 or codes.ndim != 3 or meta.ndim != 4:
+                raise ValueError("QuantKV: codes must be uint8 [Hkv, cap, d*bits/8], meta bf16 [Hkv, cap, d/group, 2]")
+            if meta.shape[:2] != codes.shape[:2] or meta.shape[3] != 2 or not meta.shape[2]:
+                raise ValueError("QuantKV: codes and meta do not match")
+            if codes.stride()[1:] != (codes.shape[2], 1) or meta.stride()[1:] != (2 * meta.shape[2], 2, 1):
+                raise ValueError("QuantKV: rows must be dense")
+        if k_codes.shape != v_codes.shape or k_meta.shape != v_meta.shape:
+            raise ValueError("QuantKV: keys and values do not match")
+        if any(t.device != k_codes.device for t in (k_meta, v_codes, v_meta)):
+            raise ValueError("QuantKV: buffers must be on one device")
+        if k_codes.shape[2] * 8 // bits % k_meta.shape[2]:
+            raise ValueError("QuantKV: group must divide head_dim")
+        self._adopt(k_codes, k_meta, v_codes, v_meta, bits)
+        return self
+
+    def _adopt(self, k_codes, k_meta, v_codes, v_meta, bits):
+        self.k_codes, self.k_meta, self.v_codes, self.v_meta, self.bits = k_codes, k_meta, v_codes, v_meta, bits
+        self.kv_heads, self.capacity = k_codes.shape[:2]
+        self.head_dim = k_codes.shape[2] * 8 // bits
+        self.group = self.head_dim // k_meta.shape[2]
+        self.device = k_codes.device
+        self._struct = _lib.QkvCache(
+            k_codes=k_codes.data_ptr(), k_meta=k_meta.data_ptr(), v_codes=v_codes.data_ptr(), v_meta=v_meta.data_ptr(),
+            k_codes_h=k_codes.stride(0), k_meta_h=k_meta.stride(0) // 2, v_codes_h=v_codes.stride(0),
+            v_meta_h=v_meta.stride(0) // 2, kv_heads=self.kv_heads, cap=self.capacity, d=self.head_dim, bits=bits,
+            group=self.group)
+        # Calls fill a copy of this, so that threads may share a cache.
+        self._attn = _lib.QkvAttnArgs(cache=self._struct)
+
+    @property
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_meta, self.v_codes, self.v_meta))
+
+    def write(self, k, v, at, *, values=False):
+        """Quantise k / v [Hkv, T, d] (fp16, bf16 or fp32) into rows at, at + 1, ...; ``at`` an int, or a
+        1-element GPU integer tensor (rows that fall outside the cache are then skipped). With
+        ``values``, returns what the rows now stand for, (k, v) [Hkv, T, d] in the input dtype, stored
+        as [T, Hkv, d]."""
+        if not k.is_cuda or k.device != self.device or v.device != self.device:
+            raise ValueError("QuantKV.write requires CUDA tensors on the cache's device")
+        if k.dtype not in _ops._DT or v.dtype != k.dtype:
+            raise ValueError("QuantKV.write: k and v must share one of f16/bf16/f32")
+        if k.ndim != 3 or k.shape != v.shape or k.shape[0] != self.kv_heads or k.shape[2] != self.head_dim:
+            raise ValueError("QuantKV.write: k and v must be [Hkv, T, d] of the cache")
+        hk, t, d = k.shape
+        k, v = _ops.rows_view(k), _ops.rows_view(v)
+        a = _lib.QkvWriteArgs(cache=self._struct, k=k.data_ptr(), sk_h=k.stride(0), sk_t=k.stride(1), v=v.data_ptr(),
+                              sv_h=v.stride(0), sv_t=v.stride(1), t=t, dtype=_ops._DT[k.dtype])
+        keep = None
+        if isinstance(at, torch.Tensor):
+            keep = _ops._n_arg(at, 0, self.device)[2]
+            a.at_dev = keep.data_ptr()
+        else:
+            a.at = int(at)
+            if a.at < 0 or a.at + t > self.capacity:
+                raise ValueError(f"QuantKV.write: rows [{a.at}, {a.at + t}) outside a cache of {self.capacity}")
+        out = None
+        if values:
+            both = torch.empty((2, t, hk, d), dtype=k.dtype, device=self.device)
+            out = both[0].transpose(0, 1), both[1].transpose(0, 1)
+            a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
+            a.sok_h = a.sov_h = d
+            a.sok_t = a.sov_t = hk * d
+        _lib.check(_lib.lib().bb_qkv_write(C.byref(a), _ops._stream(k)), "QuantKV.write")
+        del keep
+        return out
+
+    def read(self, positions=None, *, start=0, stop=None, dtype=torch.bfloat16):
+        """Values of rows [start, stop), or of rows ``positions`` (int32 / int64 [Hkv, L]; positions outside the
+        cache give zeros): (k, v) [Hkv, L, d]."""
+        if dtype not in _ops._DT:
+            raise ValueError("QuantKV.read: dtype must be one of f16/bf16/f32")
+        a = _lib.QkvReadArgs(cache=self._struct, dtype=_ops._DT[dtype])
+        if positions is None:
+            stop = self.capacity if stop is None else int(stop)
+            if not 0 <= start <= stop <= self.capacity:
+                raise ValueError(f"QuantKV.read: rows [{start}, {stop}) outside a cache of {self.capacity}")
+            a.start, rows = start, stop - start
+        else:
+            if positions.device != self.device or positions.dtype not in (torch.int32, torch.int64):
+                raise ValueError("QuantKV.read: positions must be int32 or int64 on the cache's device")
+            if positions.ndim != 2 or positions.shape[0] != self.kv_heads:
+                raise ValueError("QuantKV.read: positions must be [Hkv, L]")
+            rows = positions.shape[1]
+            if positions.stride(-1) != 1:
+                positions = positions.contiguous()
+            a.positions = positions.data_ptr() if rows else None
+            a.sp_h, a.pos_i64 = positions.stride(0), int(positions.dtype == torch.int64)
+        hk, d = self.kv_heads, self.head_dim
+        both = torch.empty((2, hk, rows, d), dtype=dtype, device=self.device)
+        if not rows:
+            return both[0], both[1]
+        a.rows = rows
+        a.out_k, a.out_v = both.data_ptr(), both[1].data_ptr()
+        a.sok_h = a.sov_h = rows * d
+        a.sok_t = a.sov_t = d
+        _lib.check(_lib.lib().bb_qkv_read(C.byref(a), _ops._stream(self.k_codes)), "QuantKV.read")
+        return both[0], both[1]
+
+
+def _args(q, kv, front, window, scale, n, splits, what):
+    """The filled argument struct of an attention call, and the tensors that must outlive it."""
+    if not q.is_cuda or q.dtype not in _HALF:
+        raise ValueError(f"{what} requires CUDA FP16/BF16 queries")
+    if q.device != kv.device:
+        raise ValueError(f"{what}: q and the cache must be on one device")
+    if q.shape[0] % kv.kv_heads or not q.shape[0] or q.shape[-1] != kv.head_dim:
+        raise ValueError(f"{what}: q must be [H, ..., {kv.head_dim}] with H a multiple of {kv.kv_heads}")
+    if front < 0 or window < 0:
+        raise ValueError(f"{what}: front and window must be >= 0")
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    a = _lib.QkvAttnArgs.from_buffer_copy(kv._attn)
+    a.q, a.sq_h, a.heads = q.data_ptr(), q.stride(0), q.shape[0]
+    a.t, a.front, a.window, a.scale, a.splits = 1, front, window, scale, splits or 0
+    a.dtype = _ops._DT[q.dtype]
+    keep = None
+    if isinstance(n, torch.Tensor):
+        a.n, a.n_dev, keep = _ops._n_arg(n, kv.capacity, kv.device)
+    else:
+        a.n = kv.capacity if n is None else int(n)
+        if not 0 <= a.n <= kv.capacity:
+            raise ValueError(f"{what}: n must lie in [0, {kv.capacity}]")
+    return a, (q, keep)
+
+
+def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=None, splits=None):
+    """Attention of the newest token, q [H, d], or of the newest T tokens, q [H, T, d], over the first ``n``
+    keys of ``kv`` (their own rows written first). The token at position p attends to [0, front),
+    [p - window + 1, p] and its ``indices`` (int32 / int64 [Hkv, R], or [H, R] for a list per query
+    head; entries outside [front, p - window] are skipped), each key of the first two once;
+    ``front=0, window=n`` is dense causal attention. ``n``: an int, a 1-element GPU integer tensor, or
+    None for the whole capacity.
+
+    Returns q's shape and dtype ([T, H, d] storage for T tokens). ``splits``: pieces that a key list is
+    cut into (default: enough to fill the GPU)."""
+    if q.ndim not in (2, 3):
+        raise ValueError("quant_decode: q must be [H, d] or [H, T, d]")
+    a, keep = _args(q, kv, front, window, scale, n, splits, "quant_decode")
+    q = keep[0]
+    if q.ndim == 3:
+        h, t, d = q.shape
+        if not t or (keep[1] is None and t > a.n):
+            raise ValueError("quant_decode: the tokens of q must be among the first n cached")
+        a.t, a.sq_t = t, q.stride(1)
+        out = torch.empty((t, h, d), dtype=q.dtype, device=q.device)
+        a.so_h, a.so_t = d, h * d
+    else:
+        h, d = q.shape
+        out = torch.empty((h, d), dtype=q.dtype, device=q.device)
+        a.so_h = d
+    a.out = out.data_ptr()
+    if indices is not None and indices.shape[-1]:
+        if indices.device != q.device or indices.dtype not in (torch.int32, torch.int64):
+            raise ValueError("quant_decode: indices must be int32 or int64 on q's device")
+        if indices.ndim != 2 or indices.shape[0] not in (kv.kv_heads, h):
+            raise ValueError("quant_decode: indices must be [Hkv, R] (pooled) or [H, R] (per head)")
+        if indices.stride(-1) != 1:
+            indices = indices.contiguous()
+        a.idx, a.si_r, a.route_rows, a.route_k = indices.data_ptr(), indices.stride(0), *indices.shape
+        a.idx_i64 = int(indices.dtype == torch.int64)
+    _launch("bb_qkv_decode", a, q, "quant_decode")
+    return out if q.ndim == 2 else out.transpose(0, 1)
+
+
+def _launch(name, a, q, what):
+    L = _lib.lib()
+    size = C.c_size_t(0)
+    ref = C.byref(a)
+    _lib.check(getattr(L, name + "_workspace_size")(ref, C.byref(size)), what)
+    ws = torch.empty(size.value, dtype=torch.uint8, device=q.device)
+    _lib.check(getattr(L, name)(ref, ws.data_ptr(), size.value, _ops._stream(q)), what)
+
+
+def quant_pooled_probs(q, kv, *, front=64, window=4096, scale=1.0, n=None, splits=None):
+    """q [H, d] -> [Hkv, capacity] fp32: the softmax probability of each of the first ``n`` keys, averaged over the
+    query heads of its KV head; -1 outside [front, n - window)."""
+    if q.ndim != 2:
+        raise ValueError("quant_pooled_probs: q must be [H, d]")
+    a, keep = _args(q, kv, front, window, scale, n, splits, "quant_pooled_probs")
+    probs = torch.empty(kv.kv_heads, kv.capacity, dtype=torch.float32, device=kv.device)
+    a.out_probs = probs.data_ptr()
+    _launch("bb_qkv_route", a, keep[0], "quant_pooled_probs")
+    return probs
+
+
+def quant_route(q, kv, k_route, *, front=64, window=4096, scale=1.0, n=None, splits=None):
+    """Positions [Hkv, k_route] (int64, ascending) of the keys with the highest pooled probabilities in
+    [front, n - window). Where that range holds fewer than k_route keys, the rest lie outside it (and
+    ``quant_decode`` with the same front and window skips them)."""
+    if q.ndim != 2:
+        raise ValueError("quant_route: q must be [H, d]")
+    if not 0 <= k_route <= kv.capacity:
+        raise ValueError("quant_route: k_route must lie in [0, capacity]")
+    a, keep = _args(q, kv, front, window, scale, n, splits, "quant_route")
+    idx = torch.empty(kv.kv_heads, k_route, dtype=torch.int64, device=kv.device)
+    if not k_route:
+        return idx
+    a.out_idx, a.so_i, a.route_k, a.out_idx_i64 = idx.data_ptr(), k_route, k_route, 1
+    _launch("bb_qkv_route", a, keep[0], "quant_route")
+    return idx
