@@ -1,7 +1,7 @@
 // Attention of the newest tokens over a quantised KV cache, and decode routing over its keys
 // (semantics: include/bb_b200.h, bb_qkv_decode and bb_qkv_route).
 //
-//   qkv_partial_kernel  up to 8 NT query rows of one KV head over one split of its key list: running max,
+//   qkv_partial_kernel  up to 4, 8 or 16 query rows of one KV head over one split of its key list: running max,
 //                       sum and P.V of the split, in fp32
 //   qkv_combine_kernel  merges the splits of a row
 //   qkv_scores_kernel   log2 scores of every key for the query heads of a KV head, and per-split softmax
@@ -35,7 +35,7 @@ size_t topk_scratch_bytes(int64_t rows, int64_t n, int64_t k);
 
 namespace {
 
-constexpr int WARPS = 8;
+constexpr int SCORE_WARPS = 8, SCORE_STAGES = 3;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float M_NONE = -1.7e38f;   // running maximum before any key (finite: exp2(-inf - M_NONE) is 0)
 constexpr float LAZY = 4.f;          // the running maximum moves only when a score exceeds it by 2^4
@@ -52,6 +52,7 @@ struct AttnParams {
   const int64_t* n_dev;
   int64_t n, cap, front, window;
   int d, heads, groups, t, cols, gp, splits, ztiles, dtype;
+  int q16;          // query rows on 16-byte boundaries
   float scale_log2;
   float2* part_ml;  // [heads * t][splits] (max in log2 units, sum); routing: [heads][splits]
   float* part_acc;  // [heads * t][splits][d]
@@ -66,43 +67,47 @@ __device__ __forceinline__ int64_t cache_len(const AttnParams& p) {
   return n < 0 ? 0 : (n > p.cap ? p.cap : n);
 }
 
-// The key list of one KV head, as tiles of 16: front keys [0, fa), window keys [b0, n) of any of the
-// tokens, and lists (one, or one for each query head).
-struct Tiles {
+// The key list of one KV head in steps of 32 keys (two tiles of 16): front keys [0, fa), window keys
+// [b0, n) of any of the tokens, and lists (one, or one for each query head).
+struct Steps {
   int n, fa, b0, na, nb, nc, total;
-  __device__ __forceinline__ Tiles(const AttnParams& p, bool all) {
+  __device__ __forceinline__ Steps(const AttnParams& p, bool all) {
     const int64_t len = cache_len(p);
     n = (int)len;
     const int64_t f = all ? 0 : (p.front < len ? p.front : len);
     const int64_t w = all ? 0 : max(f, len - p.t + 1 - p.window);
     fa = (int)f;
     b0 = (int)min(w, len);
-    na = (fa + 15) / 16;
-    nb = (n - b0 + 15) / 16;
-    nc = all ? 0 : (int)((p.route_k + 15) / 16);
+    na = (fa + 31) / 32;
+    nb = (n - b0 + 31) / 32;
+    nc = all ? 0 : (int)((p.route_k + 31) / 32);
     total = na + nb + nc * (p.per_head ? p.groups : 1);
   }
+  __device__ __forceinline__ bool listed(int u) const { return u >= na + nb; }
+  __device__ __forceinline__ int base(int u) const { return u < na ? u * 32 : b0 + (u - na) * 32; }
+  __device__ __forceinline__ int end(int u) const { return u < na ? fa : n; }
 };
 
 template <int BITS, int G, int NG, bool WITH_V> struct Stage {
   static constexpr int ROW = G * 4 * BITS;                // bytes of codes a row
   static constexpr int META = NG * 4;                     // bytes of (step, low) pairs a row
-  static constexpr int K = 0, V = 16 * ROW;
-  static constexpr int KM = (WITH_V ? 2 : 1) * 16 * ROW, VM = KM + 16 * META;
-  static constexpr int POS = KM + (WITH_V ? 2 : 1) * 16 * META;
-  static constexpr int BYTES = POS + (WITH_V ? 64 : 0);
-  static_assert(BYTES % 16 == 0, "stages start on 16-byte boundaries");
+  static constexpr int SIDES = WITH_V ? 2 : 1;
+  static constexpr int V = 32 * ROW, KM = SIDES * 32 * ROW;  // K codes at 0
+  static constexpr int VM = KM + (SIDES - 1) * 32 * META;
+  static constexpr int POS = VM + 32 * META;
+  static constexpr int BYTES = POS + (WITH_V ? 128 : 0);
+  static_assert(BYTES % 16 == 0 && V <= KM && VM < BYTES, "stages start on 16-byte boundaries");
 };
 
 // Key j of a tile feeds row slot(j) of the K product, so that the keys of a thread's V operands
 // (slots 2c, 2c + 1, 2c + 8, 2c + 9) are the tile's rows c, c + 4, c + 8, c + 12, whose reads from shared
 // memory fall into different banks.
-__device__ __forceinline__ int slot_of(int j) { return (j & 8) | ((j & 3) << 1) | ((j >> 2) & 1); }
+__device__ __forceinline__ int slot_of(int j) { return (j & 24) | ((j & 3) << 1) | ((j >> 2) & 1); }
 __device__ __forceinline__ int key_of(int r) { return ((r & 1) << 2) | (r >> 1); }  // r < 8
 
 // 16-byte chunks of a staged row are stored at chunk ^ swizzle(row), against bank conflicts: K reads take a
 // quarter row a thread, V reads an eighth of rows c.
-template <int ROW> __device__ __forceinline__ int k_swizzle(int slot) { return ROW == 128 ? (slot & 1) : 0; }
+template <int ROW> __host__ __device__ __forceinline__ constexpr int k_swizzle(int slot) { return ROW == 128 ? (slot & 1) : 0; }
 template <int ROW> __device__ __forceinline__ int v_swizzle(int row) {
   return ROW == 128 ? (row & 3) << 1 : (ROW == 64 ? row & 2 : 0);
 }
@@ -114,55 +119,83 @@ template <int N> __device__ __forceinline__ void cp_async_n(uint32_t dst, const 
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0));
 }
 
-// Copies tile `tau` of the key list into a stage (asynchronous; rows that are no keys become zeros).
-template <int BITS, int G, int NG, bool WITH_V>
-__device__ __forceinline__ void fetch(const AttnParams& p, const Tiles& tl, int tau, uint32_t st, int64_t kv, int lane) {
+// A warp's view of its KV head's buffers, and the copies of a step of 32 keys into a stage. Whole steps of
+// consecutive rows, nearly all of them, take the short way: one address a buffer, constant offsets.
+template <int BITS, int G, int NG, bool WITH_V> struct Source {
   using S = Stage<BITS, G, NG, WITH_V>;
-  constexpr int CH = S::ROW / 16;  // chunks a row
-  const unsigned char* kc = p.kc + kv * p.kc_h;
-  const unsigned char* vc = WITH_V ? p.vc + kv * p.vc_h : nullptr;
-  int mine;   // position of row lane % 16, or -1
-  int base = 0;
-  const bool listed = WITH_V && tau >= tl.na + tl.nb;
-  if (!listed) {
-    const bool a = tau < tl.na;
-    base = a ? tau * 16 : tl.b0 + (tau - tl.na) * 16;
-    mine = base + lane % 16;
-    if (mine >= (a ? tl.fa : tl.n)) mine = -1;
-  } else {
-    const int u = tau - tl.na - tl.nb;
-    const int list = u / tl.nc;
-    const int64_t j = (int64_t)(u - list * tl.nc) * 16 + lane % 16;
+  static constexpr int CH = S::ROW / 16;       // 16-byte chunks a row
+  static constexpr bool FLAT = 32 % CH == 0;   // a thread's chunks lie 512 bytes apart at one place in their rows
+  const unsigned char *kc, *vc;                // + lane * 16
+  const uint32_t *km, *vm;                     // + lane * NG
+  uint32_t kdst, vdst, mdst;
+
+  __device__ __forceinline__ Source(const AttnParams& p, int64_t kv, int lane) {
+    kc = p.kc + kv * p.kc_h + lane * 16;
+    km = p.km + kv * p.km_h + lane * NG;
+    if constexpr (WITH_V) {
+      vc = p.vc + kv * p.vc_h + lane * 16;
+      vm = p.vm + kv * p.vm_h + lane * NG;
+    }
+    const int j = lane / CH, ch = lane % CH;
+    kdst = slot_of(j) * S::ROW + ((ch ^ k_swizzle<S::ROW>(slot_of(j))) << 4);
+    vdst = S::V + j * S::ROW + ((ch ^ v_swizzle<S::ROW>(j)) << 4);
+    mdst = S::KM + slot_of(lane) * S::META;
+  }
+
+  __device__ __forceinline__ void meta(uint32_t st, int64_t pos, bool ok) const {
+    constexpr int N = NG == 3 ? 4 : S::META;
+#pragma unroll
+    for (int i = 0; i < S::META / N; ++i) {
+      cp_async_n<N>(st + mdst + i * N, km + pos * NG + i, ok);
+      if constexpr (WITH_V) cp_async_n<N>(st + mdst + (S::VM - S::KM) + i * N, vm + pos * NG + i, ok);
+    }
+  }
+
+  __device__ __forceinline__ void whole(uint32_t st, int base) const {
+    const unsigned char* k = kc + (int64_t)base * S::ROW;
+    const unsigned char* v = WITH_V ? vc + (int64_t)base * S::ROW : nullptr;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      // rows 32 / CH * i further on: 8 i or 16 i slots, or (CH = 8) 4 i rows: slots 8 (i / 2) + i % 2
+      const uint32_t at = CH == 8 ? (kdst ^ (i & 1 ? 16u : 0u)) + (i >> 1) * 8 * S::ROW + (i & 1) * S::ROW : kdst + i * 512;
+      cp_async_16(st + at, k + i * 512, true);
+      if constexpr (WITH_V) cp_async_16(st + vdst + i * 512, v + i * 512, true);
+    }
+    meta(st, base, true);
+  }
+
+  // Rows at `mine` (a position a lane, -1: none, filled with zeros).
+  __device__ __forceinline__ void rows(uint32_t st, int mine, int lane) const {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int x = lane + 32 * i, j = x / CH, ch = x % CH, sl = slot_of(j);
+      const int pos = __shfl_sync(0xffffffffu, mine, j);
+      const int64_t off = (int64_t)(pos < 0 ? 0 : pos) * S::ROW + (ch - lane) * 16;
+      cp_async_16(st + sl * S::ROW + ((ch ^ k_swizzle<S::ROW>(sl)) << 4), kc + off, pos >= 0);
+      if constexpr (WITH_V) cp_async_16(st + S::V + j * S::ROW + ((ch ^ v_swizzle<S::ROW>(j)) << 4), vc + off, pos >= 0);
+    }
+    meta(st, (mine < 0 ? 0 : mine) - lane, mine >= 0);
+  }
+
+  __device__ __forceinline__ void fetch(const AttnParams& p, const Steps& sp, int u, uint32_t st, int64_t kv, int lane) const {
+    if (!WITH_V || !sp.listed(u)) {
+      const int base = sp.base(u), end = sp.end(u);
+      if (FLAT && base + 32 <= end) whole(st, base);
+      else rows(st, base + lane < end ? base + lane : -1, lane);
+      return;
+    }
+    const int w = u - sp.na - sp.nb, list = w / sp.nc;
+    const int64_t j = (int64_t)(w - list * sp.nc) * 32 + lane;
     int64_t pos = -1;
     if (j < p.route_k) {
       const int64_t o = (p.per_head ? kv * p.groups + list : kv) * p.si_r + j;
       pos = p.idx64 ? static_cast<const int64_t*>(p.idx)[o] : (int64_t) static_cast<const int32_t*>(p.idx)[o];
     }
-    mine = (pos >= tl.fa && pos < tl.n) ? (int)pos : -1;
-    if (lane < 16) asm volatile("st.shared.s32 [%0], %1;" ::"r"(st + S::POS + slot_of(lane) * 4), "r"(mine) : "memory");
+    const int mine = (pos >= sp.fa && pos < sp.n) ? (int)pos : -1;
+    asm volatile("st.shared.s32 [%0], %1;" ::"r"(st + S::POS + slot_of(lane) * 4), "r"(mine) : "memory");
+    rows(st, mine, lane);
   }
-#pragma unroll
-  for (int i = 0; i < (16 * CH + 31) / 32; ++i) {
-    const int x = lane + 32 * i;
-    const int j = x / CH, ch = x % CH;
-    const int pos = __shfl_sync(0xffffffffu, mine, j & 15);
-    if (16 * CH % 32 == 0 || x < 16 * CH) {
-      const int64_t off = (int64_t)(pos < 0 ? 0 : pos) * S::ROW + ch * 16;
-      const int sl = slot_of(j);
-      cp_async_16(st + S::K + sl * S::ROW + ((ch ^ k_swizzle<S::ROW>(sl)) << 4), kc + off, pos >= 0);
-      if constexpr (WITH_V)
-        cp_async_16(st + S::V + j * S::ROW + ((ch ^ v_swizzle<S::ROW>(j)) << 4), vc + off, pos >= 0);
-    }
-  }
-  if (WITH_V || lane < 16) {
-    const bool second = lane >= 16;
-    const uint32_t* meta = (second ? p.vm + kv * p.vm_h : p.km + kv * p.km_h) + (int64_t)(mine < 0 ? 0 : mine) * NG;
-    const uint32_t dst = st + (second ? S::VM : S::KM) + slot_of(lane % 16) * S::META;
-    constexpr int N = NG == 3 ? 4 : S::META;
-#pragma unroll
-    for (int i = 0; i < S::META / N; ++i) cp_async_n<N>(dst + i * N, meta + i, mine >= 0);
-  }
-}
+};
 
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t at) {
   if constexpr (N % 4 == 0) {
@@ -233,33 +266,70 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ float step_of(uint32_t m) { return __uint_as_float(m << 16); }
 __device__ __forceinline__ float low_of(uint32_t m) { return __uint_as_float(m & 0xFFFF0000u); }
 
-// The query side of a warp: operands for 8 NT columns (column = token * groups + head within the KV head's
-// query heads), and, for this thread's columns 8 nt + 2c and + 1, the sums of each group's elements and
-// the factor that turns (codes . operand) into a log2 score.
-template <int BITS, int G, int NG, int NT> struct Query {
-  uint32_t f[NT][G][2][2];
+// C += A B; A 16 x 16 codes or probabilities, fp16; and the same from C = 0.
+__device__ __forceinline__ void mma_h(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  mma_16816<__half>(d, a, b);
+}
+__device__ __forceinline__ void mma_h0(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+}
+
+// How a step's 32 keys and the query rows fill a product's 16 rows and 8 columns.
+//   SPLIT (at most 4 query rows): each k-slice of 16 holds 8 dimensions of both tiles, and the query rows
+//     stand in columns 0-3 against the first tile's dimensions and in columns 4-7 against the second's
+//     (zeros elsewhere). One product gives the scores of 32 keys, and every thread's four scores are
+//     distinct (key, query) pairs, so the softmax costs half as much as with four idle columns.
+//   else: NT column tiles of 8 query rows, the two key tiles one after the other.
+template <bool SPLIT, int NT> struct Layout {
+  static constexpr int COLS = SPLIT ? 4 : 8 * NT;   // query rows of a warp
+  static constexpr int TILES = SPLIT ? 1 : 2;       // score tiles a step
+  static_assert(!SPLIT || NT == 1, "SPLIT has one column tile");
+  // Query row of column 8 nt + 2c + k, and the key tile (of a split step) that it belongs to.
+  static __device__ __forceinline__ int col(int nt, int c, int k) { return SPLIT ? (2 * c + k) & 3 : nt * 8 + 2 * c + k; }
+  static __device__ __forceinline__ int tile(int x, int c) { return SPLIT ? c >> 1 : x; }
+};
+
+// The query side of a warp: operands for its columns (query row = token * groups + head within the KV head's
+// query heads), and, for this thread's columns, the sums of each group's elements and the factor that
+// turns (codes . operand) into a log2 score.
+template <int BITS, int G, int NG, bool SPLIT, int NT> struct Query {
+  using Y = Layout<SPLIT, NT>;
+  // four sets of dimensions a block of 32, as they come out of a word of codes: SPLIT: a product each; else two
+  // products of two sets
+  uint32_t f[NT][G][SPLIT ? 4 : 2][2];
   float sum[NT][NG][2], mul[NT][2];
 
   __device__ __forceinline__ void load(const AttnParams& p, int64_t kv, int col0, int lane) {
     const int r = lane / 4, c = lane % 4;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int col = col0 + nt * 8 + r;
+      const int col = col0 + (SPLIT ? r & 3 : nt * 8 + r);
+      const bool live = col < p.cols;
       float x[G][8];
       float top = 0.f;
-      const int64_t at = col < p.cols ? (kv * p.groups + col % p.groups) * p.sq_h + (int64_t)(col / p.groups) * p.sq_t : 0;
+      const int64_t at = live ? (kv * p.groups + col % p.groups) * p.sq_h + (int64_t)(col / p.groups) * p.sq_t : 0;
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+      for (int g = 0; g < G; ++g) {
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) + at + g * 32 + c * 8;
+        if (live && p.q16) {
+          raw = *reinterpret_cast<const uint4*>(src);
+        } else if (live) {
+          uint16_t* e = reinterpret_cast<uint16_t*>(&raw);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = src[i];
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int64_t e = at + g * 32 + c * 8 + i;
-          float v = 0.f;
-          if (col < p.cols)
-            v = p.dtype == BB_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[e])
-                                   : __half2float(static_cast<const __half*>(p.q)[e]);
-          x[g][i] = v;
-          top = fmaxf(top, fabsf(v));
+          const uint32_t w = i < 2 ? raw.x : (i < 4 ? raw.y : (i < 6 ? raw.z : raw.w));
+          const uint16_t h = (uint16_t)(i % 2 ? w >> 16 : w);
+          x[g][i] = p.dtype == BB_BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+          top = fmaxf(top, fabsf(x[g][i]));
         }
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^e with top 2^e in [2^10, 2^11)
@@ -273,21 +343,27 @@ template <int BITS, int G, int NG, int NT> struct Query {
       for (int g = 0; g < G; ++g) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[g / (G / NG)] += x[g][i];
-        // In the order in which codes come out of a word: 4 bits: (0,4) (2,6) at 2^-24 and (1,5) (3,7) at
-        // 2^-20; 8 bits: (0,2) (1,3) and (4,6) (5,7), all at 2^-24.
-        if constexpr (BITS == 4) {
-          const float up16 = up * 16.f;
-          f[nt][g][0][0] = pack2<__half>(x[g][0] * up16, x[g][4] * up16);
-          f[nt][g][0][1] = pack2<__half>(x[g][2] * up16, x[g][6] * up16);
-          f[nt][g][1][0] = pack2<__half>(x[g][1] * up, x[g][5] * up);
-          f[nt][g][1][1] = pack2<__half>(x[g][3] * up, x[g][7] * up);
-        } else {
-          const float up16 = up * 16.f;
+        // Sets of dimensions in the order in which codes come out of a word. 4 bits: (0,4) (1,5) (2,6) (3,7), the
+        // even sets at 2^-24 and the odd ones at 2^-20; 8 bits: (0,2) (1,3) (4,6) (5,7), all at 2^-24.
+        uint32_t h[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            f[nt][g][h][0] = pack2<__half>(x[g][4 * h] * up16, x[g][4 * h + 2] * up16);
-            f[nt][g][h][1] = pack2<__half>(x[g][4 * h + 1] * up16, x[g][4 * h + 3] * up16);
+        for (int k = 0; k < 4; ++k) {
+          const int i0 = BITS == 4 ? k : (k / 2) * 4 + k % 2, i1 = BITS == 4 ? k + 4 : i0 + 2;
+          const float w = BITS == 4 && k % 2 ? up : up * 16.f;
+          h[k] = pack2<__half>(x[g][i0] * w, x[g][i1] * w);
+        }
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            f[nt][g][k][0] = r < 4 ? h[k] : 0u;
+            f[nt][g][k][1] = r < 4 ? 0u : h[k];
           }
+        } else if constexpr (BITS == 4) {
+          f[nt][g][0][0] = h[0]; f[nt][g][0][1] = h[2];
+          f[nt][g][1][0] = h[1]; f[nt][g][1][1] = h[3];
+        } else {
+          f[nt][g][0][0] = h[0]; f[nt][g][0][1] = h[1];
+          f[nt][g][1][0] = h[2]; f[nt][g][1][1] = h[3];
         }
       }
 #pragma unroll
@@ -305,343 +381,436 @@ template <int BITS, int G, int NG, int NT> struct Query {
   }
 };
 
-// Scores of a staged tile before the columns' factors: s[nt] = (key r, columns 2c, 2c + 1), (key r + 8, ...)
-// by slot.
-template <int BITS, int G, int NG, int NT>
-__device__ __forceinline__ void tile_scores(const Query<BITS, G, NG, NT>& q, uint32_t rows, uint32_t meta, int lane,
-                                            float (&s)[NT][4]) {
-  constexpr int WPB = BITS / 4;  // words a block of 32 dimensions
-  const int r = lane / 4, c = lane % 4;
-  uint32_t w0[G * WPB], w1[G * WPB], m0[NG], m1[NG];
-  k_words<BITS, G>(w0, rows, r, c);
-  k_words<BITS, G>(w1, rows, r + 8, c);
-  lds_words(m0, meta + r * NG * 4);
-  lds_words(m1, meta + (r + 8) * NG * 4);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
-#pragma unroll
-  for (int gi = 0; gi < NG; ++gi) {
-    float acc[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
-#pragma unroll
-    for (int b = 0; b < G / NG; ++b) {
-      const int g = gi * (G / NG) + b;
-      uint32_t a[2][4];
-      if constexpr (BITS == 4) {
-        const uint32_t x0 = w0[g], x1 = w1[g], y0 = x0 >> 8, y1 = x1 >> 8;
-        a[0][0] = x0 & 0x000F000Fu; a[0][1] = x1 & 0x000F000Fu; a[0][2] = y0 & 0x000F000Fu; a[0][3] = y1 & 0x000F000Fu;
-        a[1][0] = x0 & 0x00F000F0u; a[1][1] = x1 & 0x00F000F0u; a[1][2] = y0 & 0x00F000F0u; a[1][3] = y1 & 0x00F000F0u;
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x0 = w0[2 * g + h], x1 = w1[2 * g + h];
-          a[h][0] = x0 & 0x00FF00FFu; a[h][1] = x1 & 0x00FF00FFu;
-          a[h][2] = (x0 >> 8) & 0x00FF00FFu; a[h][3] = (x1 >> 8) & 0x00FF00FFu;
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        mma_16816<__half>(acc[nt], a[0], q.f[nt][g][0]);
-        mma_16816<__half>(acc[nt], a[1], q.f[nt][g][1]);
-      }
-    }
-    const float s0 = step_of(m0[gi]), l0 = low_of(m0[gi]), s1 = step_of(m1[gi]), l1 = low_of(m1[gi]);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        s[nt][k] = fmaf(s0, acc[nt][k], fmaf(l0, q.sum[nt][gi][k], s[nt][k]));
-        s[nt][2 + k] = fmaf(s1, acc[nt][2 + k], fmaf(l1, q.sum[nt][gi][k], s[nt][2 + k]));
-      }
+// The four sets of a block's codes in a thread's K words.
+template <int BITS, int N> __device__ __forceinline__ uint32_t code_set(const uint32_t (&w)[N], int g, int k) {
+  if constexpr (BITS == 4) {
+    const uint32_t x = k < 2 ? w[g] : w[g] >> 8;
+    return x & (k % 2 ? 0x00F000F0u : 0x000F000Fu);
+  } else {
+    const uint32_t x = w[2 * g + k / 2];
+    return (k % 2 ? x >> 8 : x) & 0x00FF00FFu;
   }
 }
 
-// Which of this thread's (key, column) pairs of a tile count.
-template <int NT> struct Mask {
-  bool ok[NT][4];
-  // `front`: keys of [0, front) count for every token at or after them; else keys of the token's window.
-  __device__ __forceinline__ void range(const AttnParams& p, const Tiles& tl, int tau, int col0, int lane) {
-    const bool front = tau < tl.na;
-    const int base = front ? tau * 16 : tl.b0 + (tau - tl.na) * 16;
-    const int end = front ? tl.fa : tl.n;
+// Scores of a staged step before the columns' factors: s[x * NT + nt] = (slot r, columns 2c, 2c + 1),
+// (slot r + 8, ...) of key tile Layout::tile(x, c).
+template <int BITS, int G, int NG, bool SPLIT, int NT>
+__device__ __forceinline__ void step_scores(const Query<BITS, G, NG, SPLIT, NT>& q, uint32_t rows, uint32_t meta, int lane,
+                                            float (&s)[Layout<SPLIT, NT>::TILES * NT][4]) {
+  using Y = Layout<SPLIT, NT>;
+  const int r = lane / 4, c = lane % 4;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+  for (int x = 0; x < Y::TILES; ++x) {
+    uint32_t w[SPLIT ? 4 : 2][G * BITS / 4], m0[NG], m1[NG];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int pos = base + key_of(lane / 4) + (i / 2) * 8;
-        const int own = tl.n - p.t + (col0 + nt * 8 + 2 * (lane % 4) + (i & 1)) / p.groups;
-        ok[nt][i] = pos < end && pos <= own && (front || pos > own - p.window);
+    for (int i = 0; i < (SPLIT ? 4 : 2); ++i) k_words<BITS, G>(w[i], rows, x * 16 + i * 8 + r, c);
+    lds_words(m0, meta + (Y::tile(x, c) * 16 + r) * NG * 4);
+    lds_words(m1, meta + (Y::tile(x, c) * 16 + r + 8) * NG * 4);
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi) {
+      float acc[NT][4];
+#pragma unroll
+      for (int b = 0; b < G / NG; ++b) {
+        const int g = gi * (G / NG) + b;
+#pragma unroll
+        for (int k = 0; k < (SPLIT ? 4 : 2); ++k) {
+          // SPLIT: set k of both tiles. Else: 4 bits: sets k and k + 2 (one power of two); 8 bits: 2k and 2k + 1.
+          const int k0 = SPLIT ? k : (BITS == 4 ? k : 2 * k), k1 = SPLIT ? k : (BITS == 4 ? k + 2 : 2 * k + 1);
+          uint32_t a[4];
+          a[0] = code_set<BITS>(w[0], g, k0);
+          a[1] = code_set<BITS>(w[1], g, k0);
+          a[2] = code_set<BITS>(w[SPLIT ? 2 : 0], g, k1);
+          a[3] = code_set<BITS>(w[SPLIT ? 3 : 1], g, k1);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (b == 0 && k == 0) mma_h0(acc[nt], a, q.f[nt][g][k]);
+            else mma_h(acc[nt], a, q.f[nt][g][k]);
+          }
+        }
       }
-  }
-  __device__ __forceinline__ void listed(const AttnParams& p, const Tiles& tl, int tau, uint32_t positions, int col0, int lane) {
-    const int list = (tau - tl.na - tl.nb) / tl.nc;
+      const float s0 = step_of(m0[gi]), l0 = low_of(m0[gi]), s1 = step_of(m1[gi]), l1 = low_of(m1[gi]);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      int pos;
-      asm volatile("ld.shared.s32 %0, [%1];" : "=r"(pos) : "r"(positions + (lane / 4 + half * 8) * 4));
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float(&o)[4] = s[x * NT + nt];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int col = col0 + nt * 8 + 2 * (lane % 4) + k;
-          const int own = tl.n - p.t + col / p.groups;
-          ok[nt][half * 2 + k] = pos >= 0 && pos >= p.front && pos <= own - p.window &&
-                                 (!p.per_head || col % p.groups == list);
+          o[k] = gi == 0 ? l0 * q.sum[nt][gi][k] : fmaf(l0, q.sum[nt][gi][k], o[k]);
+          o[2 + k] = gi == 0 ? l1 * q.sum[nt][gi][k] : fmaf(l1, q.sum[nt][gi][k], o[2 + k]);
+          o[k] = fmaf(s0, acc[nt][k], o[k]);
+          o[2 + k] = fmaf(s1, acc[nt][2 + k], o[2 + k]);
         }
+      }
     }
+  }
+}
+
+// Whether this thread's (key, column) pair i of score tile x counts.
+template <bool SPLIT, int NT> struct Mask {
+  using Y = Layout<SPLIT, NT>;
+  bool ok[Y::TILES * NT][4];
+  __device__ __forceinline__ void set(const AttnParams& p, const Steps& sp, int u, uint32_t positions, int col0, int lane) {
+    const int r = lane / 4, c = lane % 4;
+    const bool listed = sp.listed(u), front = u < sp.na;
+    const int list = listed ? (u - sp.na - sp.nb) / sp.nc : 0;
+#pragma unroll
+    for (int x = 0; x < Y::TILES; ++x)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = Y::tile(x, c) * 16 + half * 8;
+        int pos;
+        if (listed) {
+          asm volatile("ld.shared.s32 %0, [%1];" : "=r"(pos) : "r"(positions + (row + r) * 4));
+        } else {
+          pos = sp.base(u) + row + key_of(r);
+          if (pos >= sp.end(u)) pos = -1;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int col = col0 + Y::col(nt, c, k);
+            const int own = sp.n - p.t + col / p.groups;  // the token's own position
+            const bool in_window = pos > own - p.window;
+            const bool list_ok = pos >= p.front && !in_window && (!p.per_head || col % p.groups == list);
+            ok[x * NT + nt][half * 2 + k] = pos >= 0 && pos <= own && (listed ? list_ok : (front || in_window));
+          }
+      }
   }
 };
 
-constexpr int stages(int bytes) { return bytes > 3000 ? 3 : 4; }
-template <int BITS, int G, int NG, int NT> constexpr size_t partial_smem() {
+// Warps a CTA and stages a warp: two CTAs a SM with 168 registers a thread for up to 8 query rows, with 255 above.
+template <int NT> constexpr int warps() { return NT == 1 ? 6 : 4; }
+constexpr int stages(int bytes) { return bytes <= 6400 ? 3 : 2; }
+template <int BITS, int G, int NG, bool SPLIT, int NT> constexpr size_t partial_smem() {
   using S = Stage<BITS, G, NG, true>;
-  const size_t ring = (size_t)WARPS * stages(S::BYTES) * S::BYTES;
-  const size_t merge = (size_t)WARPS * 8 * NT * (G * 32 + 2) * 4;
+  const size_t ring = (size_t)warps<NT>() * stages(S::BYTES) * S::BYTES;
+  const size_t merge = (size_t)warps<NT>() * Layout<SPLIT, NT>::COLS * (G * 32 + 2) * 4;
   return ring > merge ? ring : merge;
 }
 
-// Grid (splits * ztiles, kv_heads). A warp owns its ring of stages and takes tiles split * WARPS + warp,
-// then every (splits * WARPS)-th: no barrier until the warps' results are merged at the end.
-template <int BITS, int G, int NG, int NT>
-__global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 2 : 1) qkv_partial_kernel(const AttnParams p) {
+// What a warp keeps of its keys: P.V by blocks of 32 dimensions and tiles of 16, sum P by group (P as rounded to
+// fp16, for the codes' centre), sum p (low + CENTRE step) and sum p of this thread's keys, the running maximum.
+//   sum_j p_j v_j = sum_j P_j (c_j - CENTRE) + sum_j p_j (low_j + CENTRE step_j):
+// about the middle code, P's rounding acts on codes of either sign as small as the values are about theirs.
+template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
+  using Y = Layout<SPLIT, NT>;
   using S = Stage<BITS, G, NG, true>;
-  constexpr int NS = stages(S::BYTES), D = G * 32;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int r = lane / 4, c = lane % 4;
-  const int64_t kv = blockIdx.y;
-  const int split = blockIdx.x / p.ztiles, col0 = (blockIdx.x % p.ztiles) * 8 * NT;
-  const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
-  const Tiles tl(p, false);
-  const int first = split * WARPS + warp, stride = p.splits * WARPS;
+  static constexpr float CENTRE = BITS == 4 ? 8.f : 128.f;
+  static constexpr int VW = (G * BITS + 7) / 8;
+  float o[NT][G][2][4];
+  float ps[NT][(NG + 1) / 2][4];   // groups 2i (rows 0-7) and 2i + 1 (rows 8-15)
+  float mid[NT][NG][2];
+  float m[NT][2], l[NT][2];
+  float bound, pscale;             // a power of two above every step so far (2^-100: none); P_SCALE / bound
 
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) {
-    const int tau = first + i * stride;
-    if (tau < tl.total) fetch<BITS, G, NG, true>(p, tl, tau, ring + i * S::BYTES, kv, lane);
-    cp_async_commit();
-  }
-  Query<BITS, G, NG, NT> q;
-  q.load(p, kv, col0, lane);
-
-  float o[NT][G][2][4];           // P.V: block, tile of 16 dimensions
-  float lows[NT][NG][2];          // sum p low, of this thread's keys
-  float m[NT][2], l[NT][2];       // running maximum (log2 units), sum p of this thread's keys
-  float bound = 7.8886090522101181e-31f;  // power of two above every step so far (2^-100: none)
-  float pscale = P_SCALE / bound;
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+        for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] = 0.f;
+      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      m[nt][k] = M_NONE;
-      l[nt][k] = 0.f;
+      for (int k = 0; k < 2; ++k) {
+        m[nt][k] = M_NONE;
+        l[nt][k] = 0.f;
 #pragma unroll
-      for (int gi = 0; gi < NG; ++gi) lows[nt][gi][k] = 0.f;
+        for (int gi = 0; gi < NG; ++gi) mid[nt][gi][k] = 0.f;
+      }
     }
+    bound = 7.8886090522101181e-31f;
+    pscale = P_SCALE / bound;
   }
 
-  int at = 0;
-  for (int tau = first; tau < tl.total; tau += stride) {
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    const int ahead = tau + (NS - 1) * stride;
-    const int to = at == 0 ? NS - 1 : at - 1;
-    if (ahead < tl.total && ahead > tau) fetch<BITS, G, NG, true>(p, tl, ahead, ring + to * S::BYTES, kv, lane);
-    cp_async_commit();
-    const uint32_t st = ring + at * S::BYTES;
-    at = at == NS - 1 ? 0 : at + 1;
-
-    float s[NT][4];
-    tile_scores<BITS, G, NG, NT>(q, st + S::K, st + S::KM, lane, s);
-
-    // Tiles whose every key counts for every token need no mask.
-    const bool listed = tau >= tl.na + tl.nb;
-    bool edge = listed;
-    if (!listed) {
-      const bool front = tau < tl.na;
-      const int base = front ? tau * 16 : tl.b0 + (tau - tl.na) * 16;
-      edge = base + 15 > tl.n - p.t || (front ? base + 16 > tl.fa : base < tl.n - p.window);
-    }
-    Mask<NT> mask;
-    if (edge) {
-      if (listed) mask.listed(p, tl, tau, st + S::POS, col0, lane);
-      else mask.range(p, tl, tau, col0, lane);
-    }
-    uint32_t vm0[NG], vm1[NG];
-    lds_words(vm0, st + S::VM + r * S::META);
-    lds_words(vm1, st + S::VM + (r + 8) * S::META);
+  // One staged step. EDGE: some (key, column) pairs do not count.
+  template <bool EDGE>
+  __device__ __forceinline__ void step(const Query<BITS, G, NG, SPLIT, NT>& q, uint32_t st, int lane,
+                                       const Mask<SPLIT, NT>& mask) {
+    const int r = lane / 4, c = lane % 4;
+    constexpr int X = Y::TILES;
+    float s[X * NT][4];
+    step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
+    uint32_t m0[X][NG], m1[X][NG];
     float smax = 0.f;
 #pragma unroll
-    for (int gi = 0; gi < NG; ++gi) smax = fmaxf(smax, fmaxf(step_of(vm0[gi]), step_of(vm1[gi])));  // NaN ignored
-
-    float x[NT][4];
+    for (int x = 0; x < X; ++x) {
+      lds_words(m0[x], st + S::VM + (Y::tile(x, c) * 16 + r) * S::META);
+      lds_words(m1[x], st + S::VM + (Y::tile(x, c) * 16 + r + 8) * S::META);
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) smax = fmax3(smax, step_of(m0[x][gi]), step_of(m1[x][gi]));  // NaN ignored
+    }
+    float e[X * NT][4];
     bool move = smax > bound;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int x = 0; x < X; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[nt][i] = fmaf(s[nt][i], q.mul[nt][i & 1], -m[nt][i & 1]);
-        if (edge && !mask.ok[nt][i]) x[nt][i] = -INFINITY;
-        move |= x[nt][i] > LAZY;
-      }
-    if (__any_sync(0xffffffffu, move)) {
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = x * NT + nt;
+          e[y][i] = fmaf(s[y][i], q.mul[nt][i & 1], -m[nt][i & 1]);
+          if (EDGE && !mask.ok[y][i]) e[y][i] = -INFINITY;
+          move |= e[y][i] > LAZY;
+        }
+    if (__any_sync(0xffffffffu, move)) {  // rare after the first steps: the references move
       const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)));
       float shrink = 1.f;
       if (top > bound) {
         const float next = __uint_as_float((__float_as_uint(top) & 0x7F800000u) + 0x00800000u);
         shrink = bound / next;
         bound = next;
-        pscale = P_SCALE / bound;
+        pscale = P_SCALE / next;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          float v0 = s[nt][k] * q.mul[nt][k], v1 = s[nt][2 + k] * q.mul[nt][k];
-          if (edge && !mask.ok[nt][k]) v0 = -INFINITY;
-          if (edge && !mask.ok[nt][2 + k]) v1 = -INFINITY;
-          float v = fmaxf(v0, v1);
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          float v = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < X; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int y = x * NT + nt, i = 2 * h + k;
+              e[y][i] = s[y][i] * q.mul[nt][k];
+              if (EDGE && !mask.ok[y][i]) e[y][i] = -INFINITY;
+              v = fmaxf(v, e[y][i]);
+            }
+#pragma unroll
+          for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
           const float next = fmaxf(m[nt][k], v);
           f[k] = fast_exp2(m[nt][k] - next);
           m[nt][k] = next;
           l[nt][k] *= f[k];
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) lows[nt][gi][k] *= f[k];
-          x[nt][k] = v0 - next;
-          x[nt][2 + k] = v1 - next;
+          for (int gi = 0; gi < NG; ++gi) mid[nt][gi][k] *= f[k];
+#pragma unroll
+          for (int x = 0; x < X; ++x) {
+            e[x * NT + nt][k] -= next;
+            e[x * NT + nt][2 + k] -= next;
+          }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] *= f[i & 1] * shrink;
+#pragma unroll
+        for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] *= f[i & 1] * shrink;
       }
     }
-
-    float pr[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pr[nt][i] = fast_exp2(x[nt][i]);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) l[nt][k] += pr[nt][k] + pr[nt][2 + k];
-
-    // V operands: rows c, c + 4 (slots 2c, 2c + 1) and c + 8, c + 12 (slots 2c + 8, 2c + 9).
-    constexpr int VW = (G * BITS + 7) / 8;
-    uint32_t va[VW], vb[VW], vc[VW], vd[VW];
-    v_words<BITS, G>(va, st + S::V, c, r);
-    v_words<BITS, G>(vb, st + S::V, c + 4, r);
-    v_words<BITS, G>(vc, st + S::V, c + 8, r);
-    v_words<BITS, G>(vd, st + S::V, c + 12, r);
-#pragma unroll
-    for (int gi = 0; gi < NG; ++gi) {
-      const float s0 = step_of(vm0[gi]) * pscale, l0 = low_of(vm0[gi]), s1 = step_of(vm1[gi]) * pscale, l1 = low_of(vm1[gi]);
-      uint32_t b[NT][2];
+    for (int x = 0; x < X; ++x)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float u[4] = {pr[nt][0] * s0, pr[nt][1] * s0, pr[nt][2] * s1, pr[nt][3] * s1};
-        float e[4] = {pr[nt][0] * l0, pr[nt][1] * l0, pr[nt][2] * l1, pr[nt][3] * l1};
-        if (edge) {  // rows that do not count may hold NaN
+        const int y = x * NT + nt;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            u[i] = mask.ok[nt][i] ? u[i] : 0.f;
-            e[i] = mask.ok[nt][i] ? e[i] : 0.f;
-          }
-        }
-        lows[nt][gi][0] += e[0] + e[2];
-        lows[nt][gi][1] += e[1] + e[3];
-        b[nt][0] = transpose8(pack2<__half>(u[0], u[1]));
-        b[nt][1] = transpose8(pack2<__half>(u[2], u[3]));
+        for (int i = 0; i < 4; ++i) e[y][i] = fast_exp2(e[y][i]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) l[nt][k] += e[y][k] + e[y][2 + k];
       }
+    uint32_t b[NG][X * NT][2];
 #pragma unroll
-      for (int bb = 0; bb < G / NG; ++bb) {
-        const int g = gi * (G / NG) + bb;
-        uint32_t a[2][4];
-        if constexpr (BITS == 4) {
-          const uint32_t sel = g % 2 ? 0x7632u : 0x5410u;
-          const uint32_t x0 = prmt(va[g / 2], vb[g / 2], sel), x1 = prmt(vc[g / 2], vd[g / 2], sel);
-          const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
-          a[0][0] = x0 & 0x000F000Fu; a[0][1] = y0 & 0x000F000Fu; a[0][2] = x1 & 0x000F000Fu; a[0][3] = y1 & 0x000F000Fu;
-          a[1][0] = x0 & 0x00F000F0u; a[1][1] = y0 & 0x00F000F0u; a[1][2] = x1 & 0x00F000F0u; a[1][3] = y1 & 0x00F000F0u;
-        } else {
+    for (int gi = 0; gi < NG; ++gi) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t sel = h ? 0x7632u : 0x5410u;
-            const uint32_t x0 = prmt(va[g], vb[g], sel), x1 = prmt(vc[g], vd[g], sel);
-            a[h][0] = x0 & 0x00FF00FFu; a[h][1] = (x0 >> 8) & 0x00FF00FFu;
-            a[h][2] = x1 & 0x00FF00FFu; a[h][3] = (x1 >> 8) & 0x00FF00FFu;
-          }
-        }
+      for (int x = 0; x < X; ++x) {
+        const float s0 = step_of(m0[x][gi]), s1 = step_of(m1[x][gi]);
+        const float h0 = fmaf(CENTRE, s0, low_of(m0[x][gi])), h1 = fmaf(CENTRE, s1, low_of(m1[x][gi]));
+        const float t0 = s0 * pscale, t1 = s1 * pscale;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_16816<__half>(o[nt][g][0], a[0], b[nt]);
-          mma_16816<__half>(o[nt][g][1], a[1], b[nt]);
+          const int y = x * NT + nt;
+          float u[4] = {e[y][0] * t0, e[y][1] * t0, e[y][2] * t1, e[y][3] * t1};
+          if constexpr (EDGE) {  // rows that do not count may hold NaN
+            float z[4] = {e[y][0] * h0, e[y][1] * h0, e[y][2] * h1, e[y][3] * h1};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              u[i] = mask.ok[y][i] ? u[i] : 0.f;
+              z[i] = mask.ok[y][i] ? z[i] : 0.f;
+            }
+            mid[nt][gi][0] += z[0] + z[2];
+            mid[nt][gi][1] += z[1] + z[3];
+          } else {
+            mid[nt][gi][0] = fmaf(e[y][0], h0, fmaf(e[y][2], h1, mid[nt][gi][0]));
+            mid[nt][gi][1] = fmaf(e[y][1], h0, fmaf(e[y][3], h1, mid[nt][gi][1]));
+          }
+          b[gi][y][0] = transpose8(pack2<__half>(u[0], u[1]));
+          b[gi][y][1] = transpose8(pack2<__half>(u[2], u[3]));
+          constexpr uint32_t ONES = 0x3C003C00u;  // fp16 1, 1
+          const uint32_t ones[4] = {gi % 2 ? 0u : ONES, gi % 2 ? ONES : 0u, gi % 2 ? 0u : ONES, gi % 2 ? ONES : 0u};
+          mma_h(ps[nt][gi / 2], ones, b[gi][y]);
         }
       }
+    }
+    // Key tile by key tile (SPLIT: the operand's columns of the other tile are zeros)
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      uint32_t w[4][VW];  // rows c, c + 4 (slots 2c, 2c + 1) and c + 8, c + 12 (slots 2c + 8, 2c + 9)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v_words<BITS, G>(w[i], st + S::V, tile * 16 + c + 4 * i, r);
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        uint32_t bt[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            bt[nt][i] = SPLIT ? ((lane < 16) == (tile == 0) ? b[gi][0][i] : 0u) : b[gi][(SPLIT ? 0 : tile) * NT + nt][i];
+#pragma unroll
+        for (int bb = 0; bb < G / NG; ++bb) {
+          const int g = gi * (G / NG) + bb;
+          uint32_t a[2][4];
+          v_operands(a, w, g);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_h(o[nt][g][0], a[0], bt[nt]);
+            mma_h(o[nt][g][1], a[1], bt[nt]);
+          }
+        }
+      }
+    }
+  }
+
+  // Operands of block g from a tile's V words.
+  static __device__ __forceinline__ void v_operands(uint32_t (&a)[2][4], const uint32_t (&w)[4][VW], int g) {
+    if constexpr (BITS == 4) {
+      const uint32_t sel = g % 2 ? 0x7632u : 0x5410u;
+      const uint32_t x0 = prmt(w[0][g / 2], w[1][g / 2], sel), x1 = prmt(w[2][g / 2], w[3][g / 2], sel);
+      const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+      a[0][0] = x0 & 0x000F000Fu; a[0][1] = y0 & 0x000F000Fu; a[0][2] = x1 & 0x000F000Fu; a[0][3] = y1 & 0x000F000Fu;
+      a[1][0] = x0 & 0x00F000F0u; a[1][1] = y0 & 0x00F000F0u; a[1][2] = x1 & 0x00F000F0u; a[1][3] = y1 & 0x00F000F0u;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t sel = h ? 0x7632u : 0x5410u;
+        const uint32_t x0 = prmt(w[0][g], w[1][g], sel), x1 = prmt(w[2][g], w[3][g], sel);
+        a[h][0] = x0 & 0x00FF00FFu; a[h][1] = (x0 >> 8) & 0x00FF00FFu;
+        a[h][2] = x1 & 0x00FF00FFu; a[h][3] = (x1 >> 8) & 0x00FF00FFu;
+      }
+    }
+  }
+
+  // Adds up over the threads that share a column; leaves the unscaled sums in o (P.V + middle), m and l.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], off);
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+#pragma unroll
+          for (int off = SPLIT ? 2 : 4; off < 32; off *= 2)
+            mid[nt][gi][k] += __shfl_xor_sync(0xffffffffu, mid[nt][gi][k], off);
+          float& sum = ps[nt][gi / 2][gi % 2 * 2 + k];
+          if (SPLIT) sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float& x = o[nt][g][t][2 * h + k];
+              if (SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 2);
+              const int gi = g / (G / NG);
+              const float undo = BITS == 4 && t == 1 ? 1048576.f : 16777216.f;
+              x = fmaf(-CENTRE, ps[nt][gi / 2][gi % 2 * 2 + k], x * undo) * (1.f / P_SCALE);
+              x = fmaf(x, bound, mid[nt][gi][k]);
+            }
+      }
+  }
+};
+
+// Grid (splits * ztiles, kv_heads). A warp owns its ring of stages and takes steps split * W + warp, then every
+// (splits * W)-th: no barrier until the warps' results are merged at the end.
+template <int BITS, int G, int NG, bool SPLIT, int NT>
+__global__ void __launch_bounds__(32 * warps<NT>(), 2) qkv_partial_kernel(const AttnParams p) {
+  using S = Stage<BITS, G, NG, true>;
+  using Y = Layout<SPLIT, NT>;
+  constexpr int NS = stages(S::BYTES), D = G * 32, W = warps<NT>();
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int64_t kv = blockIdx.y;
+  const int split = blockIdx.x / p.ztiles, col0 = (blockIdx.x % p.ztiles) * Y::COLS;
+  const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
+  const Steps sp(p, false);
+  const Source<BITS, G, NG, true> src(p, kv, lane);
+  const int first = split * W + warp, stride = p.splits * W;
+
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) {
+    const int u = first + i * stride;
+    if (u < sp.total) src.fetch(p, sp, u, ring + i * S::BYTES, kv, lane);
+    cp_async_commit();
+  }
+  Query<BITS, G, NG, SPLIT, NT> q;
+  q.load(p, kv, col0, lane);
+  Accum<BITS, G, NG, SPLIT, NT> acc;
+  acc.clear();
+  Mask<SPLIT, NT> mask;
+
+  int at = 0;
+  for (int u = first; u < sp.total; u += stride) {
+    cp_async_wait<NS - 2>();
+    __syncwarp();
+    const int ahead = u + (NS - 1) * stride;
+    if (ahead < sp.total) src.fetch(p, sp, ahead, ring + (at == 0 ? NS - 1 : at - 1) * S::BYTES, kv, lane);
+    cp_async_commit();
+    const uint32_t st = ring + at * S::BYTES;
+    at = at == NS - 1 ? 0 : at + 1;
+    // A step whose every key counts for every token needs no mask.
+    const int base = sp.base(u);
+    const bool inner = !sp.listed(u) && base + 32 <= sp.end(u) && base + 31 <= sp.n - p.t &&
+                       (u < sp.na || base >= sp.n - p.window);
+    if (inner) {
+      acc.template step<false>(q, st, lane, mask);
+    } else {
+      mask.set(p, sp, u, st + S::POS, col0, lane);
+      acc.template step<true>(q, st, lane, mask);
     }
   }
   cp_async_wait<0>();
+  acc.finish();
   __syncthreads();  // every warp is done with its ring
 
-  float* sm = reinterpret_cast<float*>(smem);       // [WARPS][8 NT] maxima, sums, then [WARPS][8 NT][D]
-  float* sl = sm + WARPS * 8 * NT;
-  float* so = sl + WARPS * 8 * NT;
+  float* sm = reinterpret_cast<float*>(smem);       // [W][COLS] maxima, sums, then [W][COLS][D]
+  float* sl = sm + W * Y::COLS;
+  float* so = sl + W * Y::COLS;
+  const int r = lane / 4, c = lane % 4;
+  if (!SPLIT || c < 2) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < 2; ++k) {
+        const int col = warp * Y::COLS + Y::col(nt, c, k);
+        if (r == 0) {
+          sm[col] = acc.m[nt][k];
+          sl[col] = acc.l[nt][k];
+        }
 #pragma unroll
-      for (int off = 4; off < 32; off *= 2) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], off);
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int gi = 0; gi < NG; ++gi)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int off = 4; off < 32; off *= 2) lows[nt][gi][k] += __shfl_xor_sync(0xffffffffu, lows[nt][gi][k], off);
-      const int col = nt * 8 + 2 * c + k;
-      if (r == 0) {
-        sm[warp * 8 * NT + col] = m[nt][k];
-        sl[warp * 8 * NT + col] = l[nt][k];
+            for (int h = 0; h < 2; ++h)  // 4 bits: tile t holds dimensions 4r + t, 4r + t + 2; 8 bits: 4r + 2t, + 1
+              so[col * D + g * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h)] = acc.o[nt][g][t][2 * h + k];
       }
-      float* row = so + (size_t)(warp * 8 * NT + col) * D;
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // 4 bits: tile 0 holds dimensions 4r, 4r + 2 at 2^-24, tile 1 4r + 1, 4r + 3 at 2^-20; 8 bits: tile t
-            // holds 4r + 2t, 4r + 2t + 1 at 2^-24.
-            const int dim = g * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h);
-            const float undo = (BITS == 4 && t == 1 ? 1048576.f : 16777216.f) / P_SCALE;
-            row[dim] = fmaf(o[nt][g][t][2 * h + k] * undo, bound, lows[nt][g / (G / NG)][k]);
-          }
-    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 8 * NT * D; i += 32 * WARPS) {
+  for (int i = threadIdx.x; i < Y::COLS * D; i += 32 * W) {
     const int col = i / D, dim = i % D;
     if (col0 + col >= p.cols) break;
     float M = M_NONE, L = 0.f, A = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm[w * 8 * NT + col]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w * Y::COLS + col]);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float e = fast_exp2(sm[w * 8 * NT + col] - M);
-      L = fmaf(e, sl[w * 8 * NT + col], L);
-      A = fmaf(e, so[(size_t)(w * 8 * NT + col) * D + dim], A);
+    for (int w = 0; w < W; ++w) {
+      const float e = fast_exp2(sm[w * Y::COLS + col] - M);
+      L = fmaf(e, sl[w * Y::COLS + col], L);
+      A = fmaf(e, so[(w * Y::COLS + col) * D + dim], A);
     }
     const int64_t row = (kv * p.groups + (col0 + col) % p.groups) * p.t + (col0 + col) / p.groups;
     const int64_t o_at = row * p.splits + split;
@@ -698,26 +867,28 @@ __global__ void __launch_bounds__(256) qkv_combine_kernel(AttnParams p) {
 }
 
 // Grid (splits * ztiles, kv_heads): the K half of qkv_partial_kernel; scores go to [kv][key][gp].
-template <int BITS, int G, int NG, int NT>
-__global__ void __launch_bounds__(32 * WARPS, 2) qkv_scores_kernel(const AttnParams p) {
+template <int BITS, int G, int NG, bool SPLIT, int NT>
+__global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const AttnParams p) {
   using S = Stage<BITS, G, NG, false>;
-  constexpr int NS = stages(S::BYTES * 2);
+  using Y = Layout<SPLIT, NT>;
+  constexpr int NS = SCORE_STAGES, W = SCORE_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float sm[WARPS][8 * NT], sl[WARPS][8 * NT];
+  __shared__ float sm[W][Y::COLS], sl[W][Y::COLS];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int r = lane / 4, c = lane % 4;
   const int64_t kv = blockIdx.y;
-  const int split = blockIdx.x / p.ztiles, col0 = (blockIdx.x % p.ztiles) * 8 * NT;
+  const int split = blockIdx.x / p.ztiles, col0 = (blockIdx.x % p.ztiles) * Y::COLS;
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
-  const Tiles tl(p, true);
-  const int first = split * WARPS + warp, stride = p.splits * WARPS;
+  const Steps sp(p, true);
+  const Source<BITS, G, NG, false> src(p, kv, lane);
+  const int first = split * W + warp, stride = p.splits * W;
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) {
-    const int tau = first + i * stride;
-    if (tau < tl.total) fetch<BITS, G, NG, false>(p, tl, tau, ring + i * S::BYTES, kv, lane);
+    const int u = first + i * stride;
+    if (u < sp.total) src.fetch(p, sp, u, ring + i * S::BYTES, kv, lane);
     cp_async_commit();
   }
-  Query<BITS, G, NG, NT> q;
+  Query<BITS, G, NG, SPLIT, NT> q;
   q.load(p, kv, col0, lane);
   float m[NT][2], l[NT][2];  // of this thread's keys
 #pragma unroll
@@ -728,38 +899,42 @@ __global__ void __launch_bounds__(32 * WARPS, 2) qkv_scores_kernel(const AttnPar
       l[nt][k] = 0.f;
     }
   int at = 0;
-  for (int tau = first; tau < tl.total; tau += stride) {
+  for (int u = first; u < sp.total; u += stride) {
     cp_async_wait<NS - 2>();
     __syncwarp();
-    const int ahead = tau + (NS - 1) * stride;
-    const int to = at == 0 ? NS - 1 : at - 1;
-    if (ahead < tl.total && ahead > tau) fetch<BITS, G, NG, false>(p, tl, ahead, ring + to * S::BYTES, kv, lane);
+    const int ahead = u + (NS - 1) * stride;
+    if (ahead < sp.total) src.fetch(p, sp, ahead, ring + (at == 0 ? NS - 1 : at - 1) * S::BYTES, kv, lane);
     cp_async_commit();
     const uint32_t st = ring + at * S::BYTES;
     at = at == NS - 1 ? 0 : at + 1;
-    float s[NT][4];
-    tile_scores<BITS, G, NG, NT>(q, st + S::K, st + S::KM, lane, s);
-    const int pos = tau * 16 + key_of(r);
+    float s[Y::TILES * NT][4];
+    step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int x = 0; x < Y::TILES; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = pos + (i / 2) * 8 < tl.n ? s[nt][i] * q.mul[nt][i & 1] : -INFINITY;
-      const int col = col0 + nt * 8 + 2 * c;
+      for (int nt = 0; nt < NT; ++nt) {
+        float(&v)[4] = s[x * NT + nt];
+        const int pos = u * 32 + Y::tile(x, c) * 16 + key_of(r);
+        const int col = col0 + Y::col(nt, c, 0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (col < p.gp && pos + h * 8 < tl.n)
-          *reinterpret_cast<float2*>(p.scores + ((kv * p.cap + pos + h * 8) * p.gp + col)) =
-              make_float2(s[nt][2 * h], s[nt][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) {
+          const bool ok = pos + h * 8 < sp.n;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float top = fmaxf(s[nt][k], s[nt][2 + k]);
-        if (top > m[nt][k] + LAZY) {
-          l[nt][k] *= fast_exp2(m[nt][k] - top);
-          m[nt][k] = top;
+          for (int k = 0; k < 2; ++k) v[2 * h + k] = ok ? v[2 * h + k] * q.mul[nt][k] : -INFINITY;
+          if (col < p.gp && ok)
+            *reinterpret_cast<float2*>(p.scores + ((kv * p.cap + pos + h * 8) * p.gp + col)) =
+                make_float2(v[2 * h], v[2 * h + 1]);
         }
-        l[nt][k] += fast_exp2(s[nt][k] - m[nt][k]) + fast_exp2(s[nt][2 + k] - m[nt][k]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float top = fmaxf(v[k], v[2 + k]);
+          if (top > m[nt][k] + LAZY) {
+            l[nt][k] *= fast_exp2(m[nt][k] - top);
+            m[nt][k] = top;
+          }
+          l[nt][k] += fast_exp2(v[k] - m[nt][k]) + fast_exp2(v[2 + k] - m[nt][k]);
+        }
       }
-    }
   }
   cp_async_wait<0>();
 #pragma unroll
@@ -768,23 +943,23 @@ __global__ void __launch_bounds__(32 * WARPS, 2) qkv_scores_kernel(const AttnPar
     for (int k = 0; k < 2; ++k) {
       float M = m[nt][k];
 #pragma unroll
-      for (int off = 4; off < 32; off *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+      for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
       float L = l[nt][k] * fast_exp2(m[nt][k] - M);
 #pragma unroll
-      for (int off = 4; off < 32; off *= 2) L += __shfl_xor_sync(0xffffffffu, L, off);
-      if (r == 0) {
-        sm[warp][nt * 8 + 2 * c + k] = M;
-        sl[warp][nt * 8 + 2 * c + k] = L;
+      for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) L += __shfl_xor_sync(0xffffffffu, L, off);
+      if (r == 0 && (!SPLIT || c < 2)) {
+        sm[warp][Y::col(nt, c, k)] = M;
+        sl[warp][Y::col(nt, c, k)] = L;
       }
     }
   __syncthreads();
   const int col = threadIdx.x;
-  if (col < 8 * NT && col0 + col < p.cols) {
+  if (col < Y::COLS && col0 + col < p.cols) {
     float M = M_NONE, L = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm[w][col]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w][col]);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) L = fmaf(fast_exp2(sm[w][col] - M), sl[w][col], L);
+    for (int w = 0; w < W; ++w) L = fmaf(fast_exp2(sm[w][col] - M), sl[w][col], L);
     p.part_ml[(kv * p.groups + col0 + col) * p.splits + split] = make_float2(M, L);
   }
 }
@@ -826,7 +1001,7 @@ __global__ void __launch_bounds__(256) qkv_pool_kernel(AttnParams p) {
 
 struct AttnPlan {
   int64_t splits, ztiles, cols, gp;
-  int nt;
+  int columns;  // 4 (SPLIT), 8 or 16 query rows a warp
   size_t ml_bytes, acc_bytes, scores_bytes, probs_bytes, topk_bytes, total;
 };
 
@@ -847,15 +1022,15 @@ int check_attn(const bb_qkv_attn_args* a, const char* what, bool need_v) {
   return BB_OK;
 }
 
-// Columns in tiles of 8 or 16, and the splits of the key list: enough CTAs for one wave at the kernels'
-// residency (two CTAs a SM with 8 columns, one with 16), no more than one tile of 16 keys a warp.
-void plan_grid(const bb_qkv_attn_args* a, int64_t tiles, AttnPlan* pl) {
+// The splits of the key list: enough CTAs for one wave at two a SM, no more than one step of 32 keys a warp. Up to 4
+// query rows share products (SPLIT), up to 8 take one column tile, more go 16 at a time.
+void plan_grid(const bb_qkv_attn_args* a, int64_t steps, bool decode, AttnPlan* pl) {
   pl->cols = a->heads / a->cache.kv_heads * a->t;
-  pl->nt = pl->cols <= 8 ? 1 : 2;
-  pl->ztiles = cdiv(pl->cols, (int64_t)8 * pl->nt);
-  const int64_t wave = (int64_t)num_sms() * (pl->nt == 1 ? 2 : 1);
-  const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, wave / (a->cache.kv_heads * pl->ztiles));
-  pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(tiles, (int64_t)WARPS), (int64_t)1024}));
+  pl->columns = pl->cols <= 4 ? 4 : (pl->cols <= 8 ? 8 : 16);
+  pl->ztiles = cdiv(pl->cols, (int64_t)pl->columns);
+  const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 16 ? warps<2>() : warps<1>());
+  const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() * 2 / (a->cache.kv_heads * pl->ztiles));
+  pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(steps, w), (int64_t)1024}));
 }
 
 int plan_decode(const bb_qkv_attn_args* a, AttnPlan* pl) {
@@ -869,7 +1044,7 @@ int plan_decode(const bb_qkv_attn_args* a, AttnPlan* pl) {
   const int64_t f = std::min(a->front, n), w = std::min(n - f, std::min(a->window, n) + a->t - 1);
   const int64_t lists = a->route_k > 0 && a->route_rows != a->cache.kv_heads ? a->heads / a->cache.kv_heads : 1;
   if (a->route_k > ((int64_t)1 << 27) / lists) return fail(BB_ERR_UNSUPPORTED, "qkv_decode: too many routed keys");
-  plan_grid(a, cdiv(f, (int64_t)16) + cdiv(w, (int64_t)16) + lists * cdiv(a->route_k, (int64_t)16), pl);
+  plan_grid(a, cdiv(f, (int64_t)32) + cdiv(w, (int64_t)32) + lists * cdiv(a->route_k, (int64_t)32), true, pl);
   const int64_t rows = a->heads * a->t;
   pl->ml_bytes = align_up((size_t)(rows * pl->splits) * 8, 256);
   pl->acc_bytes = align_up((size_t)(rows * pl->splits * a->cache.d) * 4, 256);
@@ -883,7 +1058,7 @@ int plan_route(const bb_qkv_attn_args* a, AttnPlan* pl) {
   if (a->t != 1) return fail(BB_ERR_SHAPE, "qkv_route: one token at a time");
   if (a->route_k > a->cache.cap) return fail(BB_ERR_ARG, "qkv_route: route_k must lie in [0, capacity]");
   *pl = {};
-  plan_grid(a, cdiv(a->n_dev ? a->cache.cap : a->n, (int64_t)16), pl);
+  plan_grid(a, cdiv(a->n_dev ? a->cache.cap : a->n, (int64_t)32), false, pl);
   pl->gp = align_up(pl->cols, 2);
   pl->ml_bytes = align_up((size_t)(a->heads * pl->splits) * 8, 256);
   pl->scores_bytes = align_up((size_t)(a->cache.kv_heads * pl->gp * a->cache.cap) * 4, 256);
@@ -900,6 +1075,7 @@ AttnParams make_params(const bb_qkv_attn_args* a, const AttnPlan& pl, char* ws) 
   p.vc = static_cast<const unsigned char*>(c.v_codes); p.vm = static_cast<const uint32_t*>(c.v_meta);
   p.kc_h = c.k_codes_h; p.km_h = c.k_meta_h; p.vc_h = c.v_codes_h; p.vm_h = c.v_meta_h;
   p.q = a->q; p.sq_h = a->sq_h; p.sq_t = a->sq_t;
+  p.q16 = qkv::al16(a->q) && a->sq_h % 8 == 0 && (a->t == 1 || a->sq_t % 8 == 0);
   p.idx = a->idx; p.si_r = a->si_r;
   p.route_k = a->route_k;
   p.idx64 = a->idx_i64 != 0;
@@ -920,51 +1096,52 @@ AttnParams make_params(const bb_qkv_attn_args* a, const AttnPlan& pl, char* ws) 
   return p;
 }
 
-template <bool DECODE, int BITS, int G, int NG, int NT>
+template <bool DECODE, int BITS, int G, int NG, bool SPLIT, int NT>
 int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
   const dim3 grid((unsigned)(p.splits * p.ztiles), (unsigned)kv_heads);
   if constexpr (DECODE) {
-    constexpr size_t smem = partial_smem<BITS, G, NG, NT>();
-    if (smem > 48 * 1024)
-      cudaFuncSetAttribute(qkv_partial_kernel<BITS, G, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    qkv_partial_kernel<BITS, G, NG, NT><<<grid, 32 * WARPS, smem, stream>>>(p);
+    constexpr size_t smem = partial_smem<BITS, G, NG, SPLIT, NT>();
+    auto* kernel = qkv_partial_kernel<BITS, G, NG, SPLIT, NT>;
+    if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    kernel<<<grid, 32 * warps<NT>(), smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_partial_kernel");
   } else {
-    using S = Stage<BITS, G, NG, false>;
-    constexpr size_t smem = (size_t)WARPS * stages(S::BYTES * 2) * S::BYTES;
-    if (smem > 48 * 1024)
-      cudaFuncSetAttribute(qkv_scores_kernel<BITS, G, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    qkv_scores_kernel<BITS, G, NG, NT><<<grid, 32 * WARPS, smem, stream>>>(p);
+    constexpr size_t smem = (size_t)SCORE_WARPS * SCORE_STAGES * Stage<BITS, G, NG, false>::BYTES;
+    auto* kernel = qkv_scores_kernel<BITS, G, NG, SPLIT, NT>;
+    if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    kernel<<<grid, 32 * SCORE_WARPS, smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_scores_kernel");
   }
   return BB_OK;
 }
 
 template <bool DECODE, int BITS, int G, int NG>
-int launch_nt(const AttnParams& p, int nt, int64_t kv_heads, cudaStream_t stream) {
-  return nt == 1 ? launch<DECODE, BITS, G, NG, 1>(p, kv_heads, stream) : launch<DECODE, BITS, G, NG, 2>(p, kv_heads, stream);
+int launch_columns(const AttnParams& p, int columns, int64_t kv_heads, cudaStream_t stream) {
+  if (columns == 4) return launch<DECODE, BITS, G, NG, true, 1>(p, kv_heads, stream);
+  return columns == 8 ? launch<DECODE, BITS, G, NG, false, 1>(p, kv_heads, stream)
+                      : launch<DECODE, BITS, G, NG, false, 2>(p, kv_heads, stream);
 }
 
 template <bool DECODE, int BITS>
-int launch_shape(const AttnParams& p, int pairs, int nt, int64_t kv_heads, cudaStream_t stream) {
+int launch_shape(const AttnParams& p, int pairs, int columns, int64_t kv_heads, cudaStream_t stream) {
   switch (p.d / 32 * 8 + pairs) {
-    case 1 * 8 + 1: return launch_nt<DECODE, BITS, 1, 1>(p, nt, kv_heads, stream);
-    case 2 * 8 + 1: return launch_nt<DECODE, BITS, 2, 1>(p, nt, kv_heads, stream);
-    case 2 * 8 + 2: return launch_nt<DECODE, BITS, 2, 2>(p, nt, kv_heads, stream);
-    case 3 * 8 + 1: return launch_nt<DECODE, BITS, 3, 1>(p, nt, kv_heads, stream);
-    case 3 * 8 + 3: return launch_nt<DECODE, BITS, 3, 3>(p, nt, kv_heads, stream);
-    case 4 * 8 + 1: return launch_nt<DECODE, BITS, 4, 1>(p, nt, kv_heads, stream);
-    case 4 * 8 + 2: return launch_nt<DECODE, BITS, 4, 2>(p, nt, kv_heads, stream);
-    case 4 * 8 + 4: return launch_nt<DECODE, BITS, 4, 4>(p, nt, kv_heads, stream);
+    case 1 * 8 + 1: return launch_columns<DECODE, BITS, 1, 1>(p, columns, kv_heads, stream);
+    case 2 * 8 + 1: return launch_columns<DECODE, BITS, 2, 1>(p, columns, kv_heads, stream);
+    case 2 * 8 + 2: return launch_columns<DECODE, BITS, 2, 2>(p, columns, kv_heads, stream);
+    case 3 * 8 + 1: return launch_columns<DECODE, BITS, 3, 1>(p, columns, kv_heads, stream);
+    case 3 * 8 + 3: return launch_columns<DECODE, BITS, 3, 3>(p, columns, kv_heads, stream);
+    case 4 * 8 + 1: return launch_columns<DECODE, BITS, 4, 1>(p, columns, kv_heads, stream);
+    case 4 * 8 + 2: return launch_columns<DECODE, BITS, 4, 2>(p, columns, kv_heads, stream);
+    case 4 * 8 + 4: return launch_columns<DECODE, BITS, 4, 4>(p, columns, kv_heads, stream);
     default: return fail(BB_ERR_UNSUPPORTED, "qkv attention: head_dim %d with %d groups", p.d, pairs);
   }
 }
 
 template <bool DECODE>
-int launch_attn(const bb_qkv_attn_args* a, const AttnParams& p, int nt, cudaStream_t stream) {
+int launch_attn(const bb_qkv_attn_args* a, const AttnParams& p, int columns, cudaStream_t stream) {
   const int pairs = (int)(a->cache.d / a->cache.group);
-  return a->cache.bits == 4 ? launch_shape<DECODE, 4>(p, pairs, nt, a->cache.kv_heads, stream)
-                            : launch_shape<DECODE, 8>(p, pairs, nt, a->cache.kv_heads, stream);
+  return a->cache.bits == 4 ? launch_shape<DECODE, 4>(p, pairs, columns, a->cache.kv_heads, stream)
+                            : launch_shape<DECODE, 8>(p, pairs, columns, a->cache.kv_heads, stream);
 }
 
 }  // namespace
@@ -985,7 +1162,7 @@ int qkv_decode(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_
     return fail(BB_ERR_WORKSPACE, "qkv_decode: workspace too small (%zu < %zu)", ws_bytes, pl.total);
   if (!a->q || !a->out || (a->route_k > 0 && !a->idx)) return fail(BB_ERR_ARG, "qkv_decode: null pointer");
   AttnParams p = make_params(a, pl, static_cast<char*>(ws));
-  st = launch_attn<true>(a, p, pl.nt, stream);
+  st = launch_attn<true>(a, p, pl.columns, stream);
   if (st) return st;
   qkv_combine_kernel<<<(unsigned)(a->heads * a->t), 256, 0, stream>>>(p);
   BB_CHECK_LAUNCH("qkv_combine_kernel");
@@ -1009,7 +1186,7 @@ int qkv_route(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_t
   if (!a->q || (!a->out_probs && !a->out_idx)) return fail(BB_ERR_ARG, "qkv_route: null pointer");
   char* w = static_cast<char*>(ws);
   AttnParams p = make_params(a, pl, w);
-  st = launch_attn<false>(a, p, pl.nt, stream);
+  st = launch_attn<false>(a, p, pl.columns, stream);
   if (st) return st;
   qkv_pool_kernel<<<dim3((unsigned)cdiv(a->cache.cap, (int64_t)1024), (unsigned)a->cache.kv_heads), 256,
                     (size_t)p.groups * 8, stream>>>(p);
