@@ -478,70 +478,46 @@ template <bool SPLIT, int NT> struct Mask {
   }
 };
 
-// Warps a CTA and stages a warp: two CTAs a SM with 168 registers a thread for up to 8 query rows, with 255 above.
-template <int NT> constexpr int warps() { return NT == 1 ? 6 : 4; }
-constexpr int stages(int bytes) { return bytes <= 6400 ? 3 : 2; }
+// Warps a CTA and stages a warp: two CTAs a SM, with 128 registers a thread for 4 query rows (4 bits), 168 for 8 (and
+// for 8-bit stages, twice as large), 255 for 16.
+template <int BITS, bool SPLIT, int NT> constexpr int warps() { return SPLIT && BITS == 4 ? 8 : (NT == 1 ? 6 : 4); }
+constexpr int stages(int warps, int bytes) {
+  const int fit = 113 * 1024 / (warps * bytes);
+  return fit < 2 ? 2 : (fit > 4 ? 4 : fit);
+}
 template <int BITS, int G, int NG, bool SPLIT, int NT> constexpr size_t partial_smem() {
   using S = Stage<BITS, G, NG, true>;
-  const size_t ring = (size_t)warps<NT>() * stages(S::BYTES) * S::BYTES;
-  const size_t merge = (size_t)warps<NT>() * Layout<SPLIT, NT>::COLS * (G * 32 + 2) * 4;
+  const size_t ring = (size_t)warps<BITS, SPLIT, NT>() * stages(warps<BITS, SPLIT, NT>(), S::BYTES) * S::BYTES;
+  const size_t merge = (size_t)warps<BITS, SPLIT, NT>() * Layout<SPLIT, NT>::COLS * (G * 32 + 2) * 4;
   return ring > merge ? ring : merge;
 }
 
-// What a warp keeps of its keys: P.V by blocks of 32 dimensions and tiles of 16, sum P by group (P as rounded to
-// fp16, for the codes' centre), sum p (low + CENTRE step) and sum p of this thread's keys, the running maximum.
-//   sum_j p_j v_j = sum_j P_j (c_j - CENTRE) + sum_j p_j (low_j + CENTRE step_j):
-// about the middle code, P's rounding acts on codes of either sign as small as the values are about theirs.
-template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
+// The softmax of a warp's columns: reference points that move only when a score exceeds them by 2^LAZY or a step
+// exceeds its bound, and the sum of p over this thread's keys.
+template <bool SPLIT, int NT> struct Running {
   using Y = Layout<SPLIT, NT>;
-  using S = Stage<BITS, G, NG, true>;
-  static constexpr float CENTRE = BITS == 4 ? 8.f : 128.f;
-  static constexpr int VW = (G * BITS + 7) / 8;
-  float o[NT][G][2][4];
-  float ps[NT][(NG + 1) / 2][4];   // groups 2i (rows 0-7) and 2i + 1 (rows 8-15)
-  float mid[NT][NG][2];
   float m[NT][2], l[NT][2];
-  float bound, pscale;             // a power of two above every step so far (2^-100: none); P_SCALE / bound
+  float bound, pscale;  // a power of two above every step so far (2^-100: none); P_SCALE / bound
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] = 0.f;
-#pragma unroll
-      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] = 0.f;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         m[nt][k] = M_NONE;
         l[nt][k] = 0.f;
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) mid[nt][gi][k] = 0.f;
       }
-    }
     bound = 7.8886090522101181e-31f;
     pscale = P_SCALE / bound;
   }
 
-  // One staged step. EDGE: some (key, column) pairs do not count.
+  // Scores s (before their factors) -> p in e. Returns whether the references moved: everything kept in units of
+  // p is then to be multiplied by f, and P.V by shrink as well.
   template <bool EDGE>
-  __device__ __forceinline__ void step(const Query<BITS, G, NG, SPLIT, NT>& q, uint32_t st, int lane,
-                                       const Mask<SPLIT, NT>& mask) {
-    const int r = lane / 4, c = lane % 4;
+  __device__ __forceinline__ bool update(float (&e)[Y::TILES * NT][4], const float (&s)[Y::TILES * NT][4],
+                                         const float (&mul)[NT][2], const Mask<SPLIT, NT>& mask, float smax,
+                                         float (&f)[NT][2], float& shrink) {
     constexpr int X = Y::TILES;
-    float s[X * NT][4];
-    step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
-    uint32_t m0[X][NG], m1[X][NG];
-    float smax = 0.f;
-#pragma unroll
-    for (int x = 0; x < X; ++x) {
-      lds_words(m0[x], st + S::VM + (Y::tile(x, c) * 16 + r) * S::META);
-      lds_words(m1[x], st + S::VM + (Y::tile(x, c) * 16 + r + 8) * S::META);
-#pragma unroll
-      for (int gi = 0; gi < NG; ++gi) smax = fmax3(smax, step_of(m0[x][gi]), step_of(m1[x][gi]));  // NaN ignored
-    }
-    float e[X * NT][4];
     bool move = smax > bound;
 #pragma unroll
     for (int x = 0; x < X; ++x)
@@ -550,13 +526,15 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int y = x * NT + nt;
-          e[y][i] = fmaf(s[y][i], q.mul[nt][i & 1], -m[nt][i & 1]);
+          e[y][i] = fmaf(s[y][i], mul[nt][i & 1], -m[nt][i & 1]);
           if (EDGE && !mask.ok[y][i]) e[y][i] = -INFINITY;
-          move |= e[y][i] > LAZY;
         }
-    if (__any_sync(0xffffffffu, move)) {  // rare after the first steps: the references move
+#pragma unroll
+    for (int y = 0; y < X * NT; ++y) move |= fmaxf(fmax3(e[y][0], e[y][1], e[y][2]), e[y][3]) > LAZY;
+    const bool moved = __any_sync(0xffffffffu, move);
+    if (moved) {
       const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)));
-      float shrink = 1.f;
+      shrink = 1.f;
       if (top > bound) {
         const float next = __uint_as_float((__float_as_uint(top) & 0x7F800000u) + 0x00800000u);
         shrink = bound / next;
@@ -564,8 +542,7 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
         pscale = P_SCALE / next;
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float f[2];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float v = -INFINITY;
@@ -574,31 +551,22 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int y = x * NT + nt, i = 2 * h + k;
-              e[y][i] = s[y][i] * q.mul[nt][k];
+              e[y][i] = s[y][i] * mul[nt][k];
               if (EDGE && !mask.ok[y][i]) e[y][i] = -INFINITY;
               v = fmaxf(v, e[y][i]);
             }
 #pragma unroll
           for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
           const float next = fmaxf(m[nt][k], v);
-          f[k] = fast_exp2(m[nt][k] - next);
+          f[nt][k] = fast_exp2(m[nt][k] - next);
           m[nt][k] = next;
-          l[nt][k] *= f[k];
-#pragma unroll
-          for (int gi = 0; gi < NG; ++gi) mid[nt][gi][k] *= f[k];
+          l[nt][k] *= f[nt][k];
 #pragma unroll
           for (int x = 0; x < X; ++x) {
             e[x * NT + nt][k] -= next;
             e[x * NT + nt][2 + k] -= next;
           }
         }
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] *= f[i & 1] * shrink;
-#pragma unroll
-        for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] *= f[i & 1] * shrink;
-      }
     }
 #pragma unroll
     for (int x = 0; x < X; ++x)
@@ -610,14 +578,92 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
 #pragma unroll
         for (int k = 0; k < 2; ++k) l[nt][k] += e[y][k] + e[y][2 + k];
       }
-    uint32_t b[NG][X * NT][2];
+    return moved;
+  }
+  __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int gi = 0; gi < NG; ++gi) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < X; ++x) {
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], off);
+  }
+};
+
+// P.V. Written about the middle code C,
+//   sum_j p_j v_j = sum_j P_j (c_j - C) + sum_j p_j (low_j + C step_j),   P = p step rounded to fp16,
+// so that P's rounding, and the accumulators', act on numbers as small as the values are about their middle.
+// Products with the bare codes give sum P c, products with ones sum P; every few steps C sum P is taken off.
+template <int BITS> constexpr float CENTRE = BITS == 4 ? 8.f : 128.f;
+constexpr uint32_t ONES = 0x3C003C00u;  // fp16 1, 1
+constexpr int SETTLE = 4;               // steps between two subtractions
+
+// What a power of two the codes of accumulator tile t carry: 2^-24, with 4 bits 2^-20 in the second tile.
+template <int BITS> __device__ __forceinline__ constexpr float code_unit(int t) {
+  return BITS == 4 && t == 1 ? 9.5367431640625e-07f : 5.9604644775390625e-08f;
+}
+
+// Up to 8 NT query rows in columns; a product covers 16 keys and 16 dimensions.
+template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
+  using Y = Layout<SPLIT, NT>;
+  using S = Stage<BITS, G, NG, true>;
+  static constexpr int VW = (G * BITS + 7) / 8;
+  float o[NT][G][2][4];            // block of 32 dimensions, tile of 16
+  float ps[NT][(NG + 1) / 2][4];   // sum P of groups 2i (rows 0-7) and 2i + 1 (rows 8-15)
+  float mid[NT][NG][2];            // sum p (low + C step) of this thread's keys
+  Running<SPLIT, NT> run;
+
+  __device__ __forceinline__ void clear(int) {
+    run.clear();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] = 0.f;
+#pragma unroll
+      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NG * 2; ++i) mid[nt][i / 2][i % 2] = 0.f;
+    }
+  }
+
+  template <bool EDGE>
+  __device__ __forceinline__ void step(const Query<BITS, G, NG, SPLIT, NT>& q, uint32_t st, int lane,
+                                       const Mask<SPLIT, NT>& mask) {
+    const int r = lane / 4, c = lane % 4;
+    float s[2 * NT][4], e[2 * NT][4], f[NT][2], shrink;
+    step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
+    uint32_t m0[2][NG], m1[2][NG];
+    float smax = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      lds_words(m0[x], st + S::VM + (x * 16 + r) * S::META);
+      lds_words(m1[x], st + S::VM + (x * 16 + r + 8) * S::META);
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) smax = fmax3(smax, step_of(m0[x][gi]), step_of(m1[x][gi]));  // NaN ignored
+    }
+    if (run.template update<EDGE>(e, s, q.mul, mask, smax, f, shrink)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < NG * 2; ++i) mid[nt][i / 2][i % 2] *= f[nt][i % 2];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] *= f[nt][i & 1] * shrink;
+#pragma unroll
+        for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] *= f[nt][i & 1] * shrink;
+      }
+    }
+    uint32_t b[NG][2 * NT][2];
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
         const float s0 = step_of(m0[x][gi]), s1 = step_of(m1[x][gi]);
-        const float h0 = fmaf(CENTRE, s0, low_of(m0[x][gi])), h1 = fmaf(CENTRE, s1, low_of(m1[x][gi]));
-        const float t0 = s0 * pscale, t1 = s1 * pscale;
+        const float h0 = fmaf(CENTRE<BITS>, s0, low_of(m0[x][gi])), h1 = fmaf(CENTRE<BITS>, s1, low_of(m1[x][gi]));
+        const float t0 = s0 * run.pscale, t1 = s1 * run.pscale;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int y = x * NT + nt;
@@ -637,43 +683,30 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
           }
           b[gi][y][0] = transpose8(pack2<__half>(u[0], u[1]));
           b[gi][y][1] = transpose8(pack2<__half>(u[2], u[3]));
-          constexpr uint32_t ONES = 0x3C003C00u;  // fp16 1, 1
           const uint32_t ones[4] = {gi % 2 ? 0u : ONES, gi % 2 ? ONES : 0u, gi % 2 ? 0u : ONES, gi % 2 ? ONES : 0u};
           mma_h(ps[nt][gi / 2], ones, b[gi][y]);
         }
       }
-    }
-    // Key tile by key tile (SPLIT: the operand's columns of the other tile are zeros)
 #pragma unroll
-    for (int tile = 0; tile < 2; ++tile) {
+    for (int x = 0; x < 2; ++x) {
       uint32_t w[4][VW];  // rows c, c + 4 (slots 2c, 2c + 1) and c + 8, c + 12 (slots 2c + 8, 2c + 9)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v_words<BITS, G>(w[i], st + S::V, tile * 16 + c + 4 * i, r);
+      for (int i = 0; i < 4; ++i) v_words<BITS, G>(w[i], st + S::V, x * 16 + c + 4 * i, r);
 #pragma unroll
-      for (int gi = 0; gi < NG; ++gi) {
-        uint32_t bt[NT][2];
+      for (int g = 0; g < G; ++g) {
+        uint32_t a[2][4];
+        operands(a, w, g);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            bt[nt][i] = SPLIT ? ((lane < 16) == (tile == 0) ? b[gi][0][i] : 0u) : b[gi][(SPLIT ? 0 : tile) * NT + nt][i];
-#pragma unroll
-        for (int bb = 0; bb < G / NG; ++bb) {
-          const int g = gi * (G / NG) + bb;
-          uint32_t a[2][4];
-          v_operands(a, w, g);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_h(o[nt][g][0], a[0], bt[nt]);
-            mma_h(o[nt][g][1], a[1], bt[nt]);
-          }
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_h(o[nt][g][0], a[0], b[g / (G / NG)][x * NT + nt]);
+          mma_h(o[nt][g][1], a[1], b[g / (G / NG)][x * NT + nt]);
         }
       }
     }
   }
 
-  // Operands of block g from a tile's V words.
-  static __device__ __forceinline__ void v_operands(uint32_t (&a)[2][4], const uint32_t (&w)[4][VW], int g) {
+  // Operands of block g: the codes of a dimension of two keys side by side.
+  static __device__ __forceinline__ void operands(uint32_t (&a)[2][4], const uint32_t (&w)[4][VW], int g) {
     if constexpr (BITS == 4) {
       const uint32_t sel = g % 2 ? 0x7632u : 0x5410u;
       const uint32_t x0 = prmt(w[0][g / 2], w[1][g / 2], sel), x1 = prmt(w[2][g / 2], w[3][g / 2], sel);
@@ -691,46 +724,207 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
     }
   }
 
-  // Adds up over the threads that share a column; leaves the unscaled sums in o (P.V + middle), m and l.
-  __device__ __forceinline__ void finish() {
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int gi = g / (G / NG);
+          o[nt][g][i / 4][i % 4] = fmaf(-CENTRE<BITS> * code_unit<BITS>(i / 4), ps[nt][gi / 2][gi % 2 * 2 + i % 2], o[nt][g][i / 4][i % 4]);
+        }
+#pragma unroll
+      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] = 0.f;
+    }
+  }
+
+  // Adds up over the threads that share a column, and hands every sum of this thread to put(query row, dimension).
+  template <typename F> __device__ __forceinline__ void finish(int lane, F put) {
+    settle();
+    run.finish();
+    const int r = lane / 4, c = lane % 4;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
-        for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], off);
+        for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-#pragma unroll
-          for (int off = SPLIT ? 2 : 4; off < 32; off *= 2)
-            mid[nt][gi][k] += __shfl_xor_sync(0xffffffffu, mid[nt][gi][k], off);
-          float& sum = ps[nt][gi / 2][gi % 2 * 2 + k];
-          if (SPLIT) sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        }
+          for (int off = 4; off < 32; off *= 2) mid[nt][gi][k] += __shfl_xor_sync(0xffffffffu, mid[nt][gi][k], off);
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float& x = o[nt][g][t][2 * h + k];
-              if (SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 2);
-              const int gi = g / (G / NG);
-              const float undo = BITS == 4 && t == 1 ? 1048576.f : 16777216.f;
-              x = fmaf(-CENTRE, ps[nt][gi / 2][gi % 2 * 2 + k], x * undo) * (1.f / P_SCALE);
-              x = fmaf(x, bound, mid[nt][gi][k]);
-            }
+            for (int h = 0; h < 2; ++h)  // 4 bits: tile t holds dimensions 4r + t, 4r + t + 2; 8 bits: 4r + 2t, + 1
+              put(Y::col(nt, c, k), g * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
+                  fmaf(o[nt][g][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound, mid[nt][g / (G / NG)][k]));
       }
+  }
+};
+
+// At most 4 query rows (SPLIT), d = 64 or 128. A product covers 8 keys and 16 dimensions of two blocks: the pair of
+// 16-bit operands that comes out of a word of codes holds a dimension of block 2i and one of block 2i + 1 (of
+// one key), the query rows stand in columns 0-3 for the first and in columns 4-7 for the second (zeros
+// elsewhere). All eight columns carry results, half as many accumulators as with idle ones.
+template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
+  using Y = Layout<true, 1>;
+  using S = Stage<BITS, G, NG, true>;
+  static constexpr int VW = (G * BITS + 7) / 8, PAIRS = G / 2;
+  static constexpr int NU = NG < PAIRS ? NG : PAIRS;  // groups that this thread's columns meet
+  static_assert(G % 2 == 0 && NU <= 2, "blocks come in pairs");
+  float o[PAIRS][2][4];
+  float ps[4];                     // sum P of this thread's groups 0 (rows 0-7) and 1 (rows 8-15)
+  float mid[NU][2];
+  Running<true, 1> run;
+  uint32_t sel0, sel1;             // place the first / second 16 bits of a word in this column's half
+
+  __device__ __forceinline__ void clear(int lane) {
+    run.clear();
+    sel0 = lane < 16 ? 0x4410u : 0x1044u;
+    sel1 = lane < 16 ? 0x4432u : 0x3244u;
+#pragma unroll
+    for (int i = 0; i < PAIRS * 8; ++i) o[i / 8][i / 4 % 2][i % 4] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ps[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NU * 2; ++i) mid[i / 2][i % 2] = 0.f;
+  }
+
+  template <bool EDGE>
+  __device__ __forceinline__ void step(const Query<BITS, G, NG, true, 1>& q, uint32_t st, int lane, const Mask<true, 1>& mask) {
+    const int r = lane / 4, c = lane % 4;
+    float s[1][4], e[1][4], f[1][2], shrink;
+    step_scores<BITS, G, NG, true, 1>(q, st, st + S::KM, lane, s);
+    // (step, low) of this thread's groups: rows r and r + 8 of both tiles
+    uint32_t m[4][NU];
+    float smax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = st + S::VM + (i * 8 + r) * S::META;
+      if constexpr (NG == G) {
+#pragma unroll
+        for (int j = 0; j < NU; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(m[i][j]) : "r"(at + j * 8 + (c >> 1) * 4));
+      } else {
+        lds_words(m[i], at);
+      }
+#pragma unroll
+      for (int j = 0; j < NU; ++j) smax = fmaxf(smax, step_of(m[i][j]));  // NaN ignored
+    }
+    if (run.template update<EDGE>(e, s, q.mul, mask, smax, f, shrink)) {
+#pragma unroll
+      for (int i = 0; i < NU * 2; ++i) mid[i / 2][i % 2] *= f[0][i % 2];
+#pragma unroll
+      for (int i = 0; i < PAIRS * 8; ++i) o[i / 8][i / 4 % 2][i % 4] *= f[0][i & 1] * shrink;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ps[i] *= f[0][i & 1] * shrink;
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      // p of key tile x from the lanes that scored it (columns 0-3: tile 0, 4-7: tile 1)
+      float t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = __shfl_sync(0xffffffffu, e[0][i], x == 0 ? lane & ~2 : lane | 2);
+      bool live[4];
+      if constexpr (EDGE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) live[i] = __shfl_sync(0xffffffffu, (int)mask.ok[0][i], x == 0 ? lane & ~2 : lane | 2) != 0;
+      }
+      uint32_t w[4][VW];  // rows c, c + 4 (slots 2c, 2c + 1) and c + 8, c + 12 (slots 2c + 8, 2c + 9)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v_words<BITS, G>(w[i], st + S::V, x * 16 + c + 4 * i, r);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t b[NU][2];
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+          const uint32_t mm = m[2 * x + half][j];
+          const float sj = step_of(mm), hj = fmaf(CENTRE<BITS>, sj, low_of(mm)), tj = sj * run.pscale;
+          float u[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            u[k] = t[2 * half + k] * tj;
+            if (EDGE) {  // rows that do not count may hold NaN
+              u[k] = live[2 * half + k] ? u[k] : 0.f;
+              mid[j][k] += live[2 * half + k] ? t[2 * half + k] * hj : 0.f;
+            } else {
+              mid[j][k] = fmaf(t[2 * half + k], hj, mid[j][k]);
+            }
+          }
+          const uint32_t both = transpose8(pack2<__half>(u[0], u[1]));  // keys 2c, 2c + 1 of this column
+          b[j][0] = prmt(both, 0u, sel0);
+          b[j][1] = prmt(both, 0u, sel1);
+          const uint32_t ones[4] = {j ? 0u : ONES, j ? ONES : 0u, j ? 0u : ONES, j ? ONES : 0u};
+          mma_h(ps, ones, b[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          uint32_t a[2][4];
+          operands(a, w[2 * half], w[2 * half + 1], i);
+          mma_h(o[i][0], a[0], b[NU == PAIRS ? i : 0]);
+          mma_h(o[i][1], a[1], b[NU == PAIRS ? i : 0]);
+        }
+      }
+    }
+  }
+
+  // Operands of blocks 2i, 2i + 1 from the words of two keys.
+  static __device__ __forceinline__ void operands(uint32_t (&a)[2][4], const uint32_t (&w0)[VW], const uint32_t (&w1)[VW], int i) {
+    if constexpr (BITS == 4) {
+      const uint32_t x0 = w0[i], x1 = w1[i], y0 = x0 >> 8, y1 = x1 >> 8;
+      a[0][0] = x0 & 0x000F000Fu; a[0][1] = y0 & 0x000F000Fu; a[0][2] = x1 & 0x000F000Fu; a[0][3] = y1 & 0x000F000Fu;
+      a[1][0] = x0 & 0x00F000F0u; a[1][1] = y0 & 0x00F000F0u; a[1][2] = x1 & 0x00F000F0u; a[1][3] = y1 & 0x00F000F0u;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t sel = h ? 0x7632u : 0x5410u;
+        const uint32_t x0 = prmt(w0[2 * i], w0[2 * i + 1], sel), x1 = prmt(w1[2 * i], w1[2 * i + 1], sel);
+        a[h][0] = x0 & 0x00FF00FFu; a[h][1] = (x0 >> 8) & 0x00FF00FFu;
+        a[h][2] = x1 & 0x00FF00FFu; a[h][3] = (x1 >> 8) & 0x00FF00FFu;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int i = 0; i < PAIRS * 8; ++i) {
+      float& x = o[i / 8][i / 4 % 2][i % 4];
+      x = fmaf(-CENTRE<BITS> * code_unit<BITS>(i / 4 % 2), ps[(NU == PAIRS ? i / 8 : 0) * 2 + i % 2], x);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ps[i] = 0.f;
+  }
+
+  template <typename F> __device__ __forceinline__ void finish(int lane, F put) {
+    settle();
+    run.finish();
+    const int r = lane / 4, c = lane % 4;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int j = 0; j < NU; ++j)
+#pragma unroll
+        for (int off = 4; off < 32; off *= 2) mid[j][k] += __shfl_xor_sync(0xffffffffu, mid[j][k], off);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            put(Y::col(0, c, k), (2 * i + (c >> 1)) * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
+                fmaf(o[i][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound, mid[NU == PAIRS ? i : 0][k]));
+    }
   }
 };
 
 // Grid (splits * ztiles, kv_heads). A warp owns its ring of stages and takes steps split * W + warp, then every
 // (splits * W)-th: no barrier until the warps' results are merged at the end.
 template <int BITS, int G, int NG, bool SPLIT, int NT>
-__global__ void __launch_bounds__(32 * warps<NT>(), 2) qkv_partial_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 2) qkv_partial_kernel(const AttnParams p) {
   using S = Stage<BITS, G, NG, true>;
   using Y = Layout<SPLIT, NT>;
-  constexpr int NS = stages(S::BYTES), D = G * 32, W = warps<NT>();
+  constexpr int NS = stages(warps<BITS, SPLIT, NT>(), S::BYTES), D = G * 32, W = warps<BITS, SPLIT, NT>();
   extern __shared__ __align__(128) unsigned char smem[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int64_t kv = blockIdx.y;
@@ -749,10 +943,10 @@ __global__ void __launch_bounds__(32 * warps<NT>(), 2) qkv_partial_kernel(const 
   Query<BITS, G, NG, SPLIT, NT> q;
   q.load(p, kv, col0, lane);
   Accum<BITS, G, NG, SPLIT, NT> acc;
-  acc.clear();
+  acc.clear(lane);
   Mask<SPLIT, NT> mask;
 
-  int at = 0;
+  int at = 0, since = 0;
   for (int u = first; u < sp.total; u += stride) {
     cp_async_wait<NS - 2>();
     __syncwarp();
@@ -771,32 +965,25 @@ __global__ void __launch_bounds__(32 * warps<NT>(), 2) qkv_partial_kernel(const 
       mask.set(p, sp, u, st + S::POS, col0, lane);
       acc.template step<true>(q, st, lane, mask);
     }
+    if (++since == SETTLE) {
+      acc.settle();
+      since = 0;
+    }
   }
   cp_async_wait<0>();
-  acc.finish();
   __syncthreads();  // every warp is done with its ring
 
   float* sm = reinterpret_cast<float*>(smem);       // [W][COLS] maxima, sums, then [W][COLS][D]
   float* sl = sm + W * Y::COLS;
   float* so = sl + W * Y::COLS;
-  const int r = lane / 4, c = lane % 4;
-  if (!SPLIT || c < 2) {
+  acc.finish(lane, [&](int row, int dim, float x) { so[(warp * Y::COLS + row) * D + dim] = x; });
+  if (lane < (SPLIT ? 2 : 4)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int col = warp * Y::COLS + Y::col(nt, c, k);
-        if (r == 0) {
-          sm[col] = acc.m[nt][k];
-          sl[col] = acc.l[nt][k];
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)  // 4 bits: tile t holds dimensions 4r + t, 4r + t + 2; 8 bits: 4r + 2t, + 1
-              so[col * D + g * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h)] = acc.o[nt][g][t][2 * h + k];
+        sm[warp * Y::COLS + Y::col(nt, lane, k)] = acc.run.m[nt][k];
+        sl[warp * Y::COLS + Y::col(nt, lane, k)] = acc.run.l[nt][k];
       }
   }
   __syncthreads();
@@ -1023,12 +1210,12 @@ int check_attn(const bb_qkv_attn_args* a, const char* what, bool need_v) {
 }
 
 // The splits of the key list: enough CTAs for one wave at two a SM, no more than one step of 32 keys a warp. Up to 4
-// query rows share products (SPLIT), up to 8 take one column tile, more go 16 at a time.
+// query rows share products (SPLIT, d = 64 or 128), up to 8 take one column tile, more go 16 at a time.
 void plan_grid(const bb_qkv_attn_args* a, int64_t steps, bool decode, AttnPlan* pl) {
   pl->cols = a->heads / a->cache.kv_heads * a->t;
-  pl->columns = pl->cols <= 4 ? 4 : (pl->cols <= 8 ? 8 : 16);
+  pl->columns = pl->cols <= 4 && a->cache.d % 64 == 0 ? 4 : (pl->cols <= 8 ? 8 : 16);
   pl->ztiles = cdiv(pl->cols, (int64_t)pl->columns);
-  const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 16 ? warps<2>() : warps<1>());
+  const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 16 ? warps<4, false, 2>() : (pl->columns == 8 || a->cache.bits == 8 ? warps<8, true, 1>() : warps<4, true, 1>()));
   const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() * 2 / (a->cache.kv_heads * pl->ztiles));
   pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(steps, w), (int64_t)1024}));
 }
@@ -1103,7 +1290,7 @@ int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
     constexpr size_t smem = partial_smem<BITS, G, NG, SPLIT, NT>();
     auto* kernel = qkv_partial_kernel<BITS, G, NG, SPLIT, NT>;
     if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    kernel<<<grid, 32 * warps<NT>(), smem, stream>>>(p);
+    kernel<<<grid, 32 * warps<BITS, SPLIT, NT>(), smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_partial_kernel");
   } else {
     constexpr size_t smem = (size_t)SCORE_WARPS * SCORE_STAGES * Stage<BITS, G, NG, false>::BYTES;
@@ -1117,7 +1304,8 @@ int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
 
 template <bool DECODE, int BITS, int G, int NG>
 int launch_columns(const AttnParams& p, int columns, int64_t kv_heads, cudaStream_t stream) {
-  if (columns == 4) return launch<DECODE, BITS, G, NG, true, 1>(p, kv_heads, stream);
+  if constexpr (G % 2 == 0)
+    if (columns == 4) return launch<DECODE, BITS, G, NG, true, 1>(p, kv_heads, stream);
   return columns == 8 ? launch<DECODE, BITS, G, NG, false, 1>(p, kv_heads, stream)
                       : launch<DECODE, BITS, G, NG, false, 2>(p, kv_heads, stream);
 }
