@@ -67,25 +67,42 @@ __device__ __forceinline__ int64_t cache_len(const AttnParams& p) {
   return n < 0 ? 0 : (n > p.cap ? p.cap : n);
 }
 
-// The key list of one KV head in steps of 32 keys (two tiles of 16): front keys [0, fa), window keys
-// [b0, n) of any of the tokens, and lists (one, or one for each query head).
+// The key list of one KV head in steps of 32 keys (two tiles of 16): front keys [0, fa), keys [b0, n) in the
+// window of any of the tokens, and lists (one, or one for each query head). First come the whole steps from
+// `bf` on, of consecutive keys that all count for every token; then the rest: the front, the ends of the
+// window and the lists. Where front and window meet, all of it is one range.
 struct Steps {
-  int n, fa, b0, na, nb, nc, total;
-  __device__ __forceinline__ Steps(const AttnParams& p, bool all) {
+  int n, fa;
+  int bf, whole;
+  int lo[3], hi[3], cut[3];  // the rest of the ranges, and the step after the last of each
+  int nc, total;
+  // every_key: the first n keys, whatever front, window and lists say.
+  __device__ __forceinline__ Steps(const AttnParams& p, bool every_key) {
     const int64_t len = cache_len(p);
     n = (int)len;
-    const int64_t f = all ? 0 : (p.front < len ? p.front : len);
-    const int64_t w = all ? 0 : max(f, len - p.t + 1 - p.window);
-    fa = (int)f;
-    b0 = (int)min(w, len);
-    na = (fa + 31) / 32;
-    nb = (n - b0 + 31) / 32;
-    nc = all ? 0 : (int)((p.route_k + 31) / 32);
-    total = na + nb + nc * (p.per_head ? p.groups : 1);
+    const int64_t f = p.front < len ? p.front : len;
+    const bool all = every_key || len - p.window <= f;
+    fa = all ? 0 : (int)f;
+    const int b0 = all ? 0 : (int)min(max(f, len - p.t + 1 - p.window), len);  // first token's window
+    bf = all ? 0 : (int)min(len - p.window, len);                              // every token's window
+    const int last = max(0, n - p.t + 1);                                      // keys that every token sees: [0, last)
+    whole = max(0, last - bf) / 32;
+    lo[0] = 0;               hi[0] = fa;
+    lo[1] = b0;              hi[1] = bf;
+    lo[2] = bf + whole * 32; hi[2] = n;
+    int u = whole;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) cut[i] = u += (hi[i] - lo[i] + 31) / 32;
+    nc = every_key ? 0 : (int)((p.route_k + 31) / 32);
+    total = u + nc * (p.per_head ? p.groups : 1);
   }
-  __device__ __forceinline__ bool listed(int u) const { return u >= na + nb; }
-  __device__ __forceinline__ int base(int u) const { return u < na ? u * 32 : b0 + (u - na) * 32; }
-  __device__ __forceinline__ int end(int u) const { return u < na ? fa : n; }
+  __device__ __forceinline__ bool listed(int u) const { return u >= cut[2]; }
+  // Keys [from, to) of a step of the rest that is not listed.
+  __device__ __forceinline__ void range(int u, int& from, int& to) const {
+    const int i = u < cut[0] ? 0 : (u < cut[1] ? 1 : 2);
+    from = (i == 0 ? lo[0] + (u - whole) * 32 : (i == 1 ? lo[1] + (u - cut[0]) * 32 : lo[2] + (u - cut[1]) * 32));
+    to = i == 0 ? hi[0] : (i == 1 ? hi[1] : hi[2]);
+  }
 };
 
 template <int BITS, int G, int NG, bool WITH_V> struct Stage {
@@ -119,49 +136,71 @@ template <int N> __device__ __forceinline__ void cp_async_n(uint32_t dst, const 
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0));
 }
 
-// A warp's view of its KV head's buffers, and the copies of a step of 32 keys into a stage. Whole steps of
-// consecutive rows, nearly all of them, take the short way: one address a buffer, constant offsets.
+// A warp's copies into its stages.
 template <int BITS, int G, int NG, bool WITH_V> struct Source {
   using S = Stage<BITS, G, NG, WITH_V>;
   static constexpr int CH = S::ROW / 16;       // 16-byte chunks a row
   static constexpr bool FLAT = 32 % CH == 0;   // a thread's chunks lie 512 bytes apart at one place in their rows
-  const unsigned char *kc, *vc;                // + lane * 16
+  const unsigned char *kc, *vc;                // of this KV head, + lane * 16
   const uint32_t *km, *vm;                     // + lane * NG
+  const unsigned char *k_at, *v_at;            // the next whole step
+  const uint32_t *km_at, *vm_at;
+  int64_t ahead;                               // rows between this warp's whole steps
   uint32_t kdst, vdst, mdst;
 
-  __device__ __forceinline__ Source(const AttnParams& p, int64_t kv, int lane) {
+  __device__ __forceinline__ Source(const AttnParams& p, int64_t kv, int lane, int64_t row, int64_t rows_ahead) {
     kc = p.kc + kv * p.kc_h + lane * 16;
     km = p.km + kv * p.km_h + lane * NG;
+    k_at = kc + row * S::ROW;
+    km_at = km + row * NG;
     if constexpr (WITH_V) {
       vc = p.vc + kv * p.vc_h + lane * 16;
       vm = p.vm + kv * p.vm_h + lane * NG;
+      v_at = vc + row * S::ROW;
+      vm_at = vm + row * NG;
     }
+    ahead = rows_ahead;
     const int j = lane / CH, ch = lane % CH;
     kdst = slot_of(j) * S::ROW + ((ch ^ k_swizzle<S::ROW>(slot_of(j))) << 4);
     vdst = S::V + j * S::ROW + ((ch ^ v_swizzle<S::ROW>(j)) << 4);
     mdst = S::KM + slot_of(lane) * S::META;
   }
 
-  __device__ __forceinline__ void meta(uint32_t st, int64_t pos, bool ok) const {
+  __device__ __forceinline__ void meta(uint32_t st, const uint32_t* k, const uint32_t* v, bool ok) const {
     constexpr int N = NG == 3 ? 4 : S::META;
 #pragma unroll
     for (int i = 0; i < S::META / N; ++i) {
-      cp_async_n<N>(st + mdst + i * N, km + pos * NG + i, ok);
-      if constexpr (WITH_V) cp_async_n<N>(st + mdst + (S::VM - S::KM) + i * N, vm + pos * NG + i, ok);
+      cp_async_n<N>(st + mdst + i * N, k + i, ok);
+      if constexpr (WITH_V) cp_async_n<N>(st + mdst + (S::VM - S::KM) + i * N, v + i, ok);
     }
   }
 
-  __device__ __forceinline__ void whole(uint32_t st, int base) const {
-    const unsigned char* k = kc + (int64_t)base * S::ROW;
-    const unsigned char* v = WITH_V ? vc + (int64_t)base * S::ROW : nullptr;
+  // The next whole step: one address a buffer, constant offsets.
+  __device__ __forceinline__ void whole(uint32_t st) {
+    if constexpr (FLAT) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      // rows 32 / CH * i further on: 8 i or 16 i slots, or (CH = 8) 4 i rows: slots 8 (i / 2) + i % 2
-      const uint32_t at = CH == 8 ? (kdst ^ (i & 1 ? 16u : 0u)) + (i >> 1) * 8 * S::ROW + (i & 1) * S::ROW : kdst + i * 512;
-      cp_async_16(st + at, k + i * 512, true);
-      if constexpr (WITH_V) cp_async_16(st + vdst + i * 512, v + i * 512, true);
+      for (int i = 0; i < CH; ++i) {
+        // rows 32 / CH * i further on: 8 i or 16 i slots, or (CH = 8) 4 i rows: slots 8 (i / 2) + i % 2
+        const uint32_t at = CH == 8 ? (kdst ^ (i & 1 ? 16u : 0u)) + (i >> 1) * 8 * S::ROW + (i & 1) * S::ROW : kdst + i * 512;
+        cp_async_16(st + at, k_at + i * 512, true);
+        if constexpr (WITH_V) cp_async_16(st + vdst + i * 512, v_at + i * 512, true);
+      }
+    } else {
+      const int lane = threadIdx.x % 32;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int x = lane + 32 * i, j = x / CH, ch = x % CH, sl = slot_of(j);
+        cp_async_16(st + sl * S::ROW + ((ch ^ k_swizzle<S::ROW>(sl)) << 4), k_at + i * 512, true);
+        if constexpr (WITH_V) cp_async_16(st + S::V + j * S::ROW + ((ch ^ v_swizzle<S::ROW>(j)) << 4), v_at + i * 512, true);
+      }
     }
-    meta(st, base, true);
+    meta(st, km_at, vm_at, true);
+    k_at += ahead * S::ROW;
+    km_at += ahead * NG;
+    if constexpr (WITH_V) {
+      v_at += ahead * S::ROW;
+      vm_at += ahead * NG;
+    }
   }
 
   // Rows at `mine` (a position a lane, -1: none, filled with zeros).
@@ -174,17 +213,19 @@ template <int BITS, int G, int NG, bool WITH_V> struct Source {
       cp_async_16(st + sl * S::ROW + ((ch ^ k_swizzle<S::ROW>(sl)) << 4), kc + off, pos >= 0);
       if constexpr (WITH_V) cp_async_16(st + S::V + j * S::ROW + ((ch ^ v_swizzle<S::ROW>(j)) << 4), vc + off, pos >= 0);
     }
-    meta(st, (mine < 0 ? 0 : mine) - lane, mine >= 0);
+    const int64_t off = (int64_t)((mine < 0 ? 0 : mine) - lane) * NG;
+    meta(st, km + off, WITH_V ? vm + off : nullptr, mine >= 0);
   }
 
-  __device__ __forceinline__ void fetch(const AttnParams& p, const Steps& sp, int u, uint32_t st, int64_t kv, int lane) const {
+  // Step u >= whole.
+  __device__ __forceinline__ void rest(const AttnParams& p, const Steps& sp, int u, uint32_t st, int64_t kv, int lane) const {
     if (!WITH_V || !sp.listed(u)) {
-      const int base = sp.base(u), end = sp.end(u);
-      if (FLAT && base + 32 <= end) whole(st, base);
-      else rows(st, base + lane < end ? base + lane : -1, lane);
+      int from, to;
+      sp.range(u, from, to);
+      rows(st, from + lane < to ? from + lane : -1, lane);
       return;
     }
-    const int w = u - sp.na - sp.nb, list = w / sp.nc;
+    const int w = u - sp.cut[2], list = w / sp.nc;
     const int64_t j = (int64_t)(w - list * sp.nc) * 32 + lane;
     int64_t pos = -1;
     if (j < p.route_k) {
@@ -195,7 +236,49 @@ template <int BITS, int G, int NG, bool WITH_V> struct Source {
     asm volatile("st.shared.s32 [%0], %1;" ::"r"(st + S::POS + slot_of(lane) * 4), "r"(mine) : "memory");
     rows(st, mine, lane);
   }
+
+  __device__ __forceinline__ void fetch(const AttnParams& p, const Steps& sp, int u, uint32_t st, int64_t kv, int lane) {
+    if (u < sp.whole) whole(st);
+    else if (u < sp.total) rest(p, sp, u, st, kv, lane);
+    cp_async_commit();
+  }
 };
+
+// Runs a warp's steps first, first + stride, ... through its ring of NS stages: inner(stage) for whole steps, edge(u, stage)
+// for the rest. No barrier: a warp only ever waits for its own copies.
+template <int NS, typename Src, typename Inner, typename Edge>
+__device__ __forceinline__ void run_steps(const AttnParams& p, const Steps& sp, Src& src, uint32_t ring, int first, int stride,
+                                          int64_t kv, int lane, Inner inner, Edge edge) {
+  constexpr int BYTES = Src::S::BYTES;
+  int u = first;
+  int left = u < sp.whole ? (sp.whole - u + stride - 1) / stride : 0;
+  int next = u + (NS - 1) * stride;
+  int at = 0;
+  while (left > 0) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if (left > 0) {
+        cp_async_wait<NS - 2>();
+        __syncwarp();
+        src.fetch(p, sp, next, ring + (i + NS - 1) % NS * BYTES, kv, lane);
+        next += stride;
+        inner(ring + i * BYTES);
+        --left;
+        u += stride;
+        at = (i + 1) % NS;
+      }
+    }
+  }
+  for (; u < sp.total; u += stride) {
+    cp_async_wait<NS - 2>();
+    __syncwarp();
+    src.fetch(p, sp, next, ring + (at == 0 ? NS - 1 : at - 1) * BYTES, kv, lane);
+    next += stride;
+    edge(u, ring + at * BYTES);
+    at = at == NS - 1 ? 0 : at + 1;
+  }
+  cp_async_wait<0>();
+}
 
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t at) {
   if constexpr (N % 4 == 0) {
@@ -259,7 +342,7 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 // Rows 8 x 8 of 16-bit elements, transposed across the warp.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -268,13 +351,22 @@ __device__ __forceinline__ float low_of(uint32_t m) { return __uint_as_float(m &
 
 // C += A B; A 16 x 16 codes or probabilities, fp16; and the same from C = 0.
 __device__ __forceinline__ void mma_h(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  mma_16816<__half>(d, a, b);
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 __device__ __forceinline__ void mma_h0(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+}
+
+// C += ones B over 8 of k: rows 0-7 (half 0) or 8-15 (half 1) of C take the column sums of B.
+__device__ __forceinline__ void mma_sum(float (&d)[4], int half, uint32_t b) {
+  constexpr uint32_t ONES = 0x3C003C00u;  // fp16 1, 1
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(half ? 0u : ONES), "r"(half ? ONES : 0u), "r"(b));
 }
 
 // How a step's 32 keys and the query rows fill a product's 16 rows and 8 columns.
@@ -450,8 +542,10 @@ template <bool SPLIT, int NT> struct Mask {
   bool ok[Y::TILES * NT][4];
   __device__ __forceinline__ void set(const AttnParams& p, const Steps& sp, int u, uint32_t positions, int col0, int lane) {
     const int r = lane / 4, c = lane % 4;
-    const bool listed = sp.listed(u), front = u < sp.na;
-    const int list = listed ? (u - sp.na - sp.nb) / sp.nc : 0;
+    const bool listed = sp.listed(u);
+    const int list = listed ? (u - sp.cut[2]) / sp.nc : 0;
+    int from = 0, to = 0;
+    if (!listed) sp.range(u, from, to);
 #pragma unroll
     for (int x = 0; x < Y::TILES; ++x)
 #pragma unroll
@@ -461,8 +555,8 @@ template <bool SPLIT, int NT> struct Mask {
         if (listed) {
           asm volatile("ld.shared.s32 %0, [%1];" : "=r"(pos) : "r"(positions + (row + r) * 4));
         } else {
-          pos = sp.base(u) + row + key_of(r);
-          if (pos >= sp.end(u)) pos = -1;
+          pos = from + row + key_of(r);
+          if (pos >= to) pos = -1;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -472,7 +566,7 @@ template <bool SPLIT, int NT> struct Mask {
             const int own = sp.n - p.t + col / p.groups;  // the token's own position
             const bool in_window = pos > own - p.window;
             const bool list_ok = pos >= p.front && !in_window && (!p.per_head || col % p.groups == list);
-            ok[x * NT + nt][half * 2 + k] = pos >= 0 && pos <= own && (listed ? list_ok : (front || in_window));
+            ok[x * NT + nt][half * 2 + k] = pos >= 0 && pos <= own && (listed ? list_ok : (pos < p.front || in_window));
           }
       }
   }
@@ -595,7 +689,6 @@ template <bool SPLIT, int NT> struct Running {
 // so that P's rounding, and the accumulators', act on numbers as small as the values are about their middle.
 // Products with the bare codes give sum P c, products with ones sum P; every few steps C sum P is taken off.
 template <int BITS> constexpr float CENTRE = BITS == 4 ? 8.f : 128.f;
-constexpr uint32_t ONES = 0x3C003C00u;  // fp16 1, 1
 constexpr int SETTLE = 4;               // steps between two subtractions
 
 // What a power of two the codes of accumulator tile t carry: 2^-24, with 4 bits 2^-20 in the second tile.
@@ -683,8 +776,8 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
           }
           b[gi][y][0] = transpose8(pack2<__half>(u[0], u[1]));
           b[gi][y][1] = transpose8(pack2<__half>(u[2], u[3]));
-          const uint32_t ones[4] = {gi % 2 ? 0u : ONES, gi % 2 ? ONES : 0u, gi % 2 ? 0u : ONES, gi % 2 ? ONES : 0u};
-          mma_h(ps[nt][gi / 2], ones, b[gi][y]);
+          mma_sum(ps[nt][gi / 2], gi % 2, b[gi][y][0]);
+          mma_sum(ps[nt][gi / 2], gi % 2, b[gi][y][1]);
         }
       }
 #pragma unroll
@@ -855,8 +948,7 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
           const uint32_t both = transpose8(pack2<__half>(u[0], u[1]));  // keys 2c, 2c + 1 of this column
           b[j][0] = prmt(both, 0u, sel0);
           b[j][1] = prmt(both, 0u, sel1);
-          const uint32_t ones[4] = {j ? 0u : ONES, j ? ONES : 0u, j ? 0u : ONES, j ? ONES : 0u};
-          mma_h(ps, ones, b[j]);
+          mma_sum(ps, j, both);
         }
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
@@ -926,51 +1018,36 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 2) qkv_partial_
   using Y = Layout<SPLIT, NT>;
   constexpr int NS = stages(warps<BITS, SPLIT, NT>(), S::BYTES), D = G * 32, W = warps<BITS, SPLIT, NT>();
   extern __shared__ __align__(128) unsigned char smem[];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   const int64_t kv = blockIdx.y;
   const int split = blockIdx.x / p.ztiles, col0 = (blockIdx.x % p.ztiles) * Y::COLS;
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
   const Steps sp(p, false);
-  const Source<BITS, G, NG, true> src(p, kv, lane);
   const int first = split * W + warp, stride = p.splits * W;
-
+  Source<BITS, G, NG, true> src(p, kv, lane, sp.bf + (int64_t)first * 32, (int64_t)stride * 32);
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) {
-    const int u = first + i * stride;
-    if (u < sp.total) src.fetch(p, sp, u, ring + i * S::BYTES, kv, lane);
-    cp_async_commit();
-  }
+  for (int i = 0; i < NS - 1; ++i) src.fetch(p, sp, first + i * stride, ring + i * S::BYTES, kv, lane);
   Query<BITS, G, NG, SPLIT, NT> q;
   q.load(p, kv, col0, lane);
   Accum<BITS, G, NG, SPLIT, NT> acc;
   acc.clear(lane);
-  Mask<SPLIT, NT> mask;
-
-  int at = 0, since = 0;
-  for (int u = first; u < sp.total; u += stride) {
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    const int ahead = u + (NS - 1) * stride;
-    if (ahead < sp.total) src.fetch(p, sp, ahead, ring + (at == 0 ? NS - 1 : at - 1) * S::BYTES, kv, lane);
-    cp_async_commit();
-    const uint32_t st = ring + at * S::BYTES;
-    at = at == NS - 1 ? 0 : at + 1;
-    // A step whose every key counts for every token needs no mask.
-    const int base = sp.base(u);
-    const bool inner = !sp.listed(u) && base + 32 <= sp.end(u) && base + 31 <= sp.n - p.t &&
-                       (u < sp.na || base >= sp.n - p.window);
-    if (inner) {
-      acc.template step<false>(q, st, lane, mask);
-    } else {
-      mask.set(p, sp, u, st + S::POS, col0, lane);
-      acc.template step<true>(q, st, lane, mask);
-    }
-    if (++since == SETTLE) {
-      acc.settle();
-      since = 0;
-    }
-  }
-  cp_async_wait<0>();
+  int since = 0;
+  run_steps<NS>(
+      p, sp, src, ring, first, stride, kv, lane,
+      [&](uint32_t st) {
+        acc.template step<false>(q, st, lane, Mask<SPLIT, NT>());
+        if (++since == SETTLE) {
+          acc.settle();
+          since = 0;
+        }
+      },
+      [&](int u, uint32_t st) {
+        Mask<SPLIT, NT> mask;
+        mask.set(p, sp, u, st + S::POS, col0, lane);
+        acc.template step<true>(q, st, lane, mask);
+        acc.settle();
+      });
   __syncthreads();  // every warp is done with its ring
 
   float* sm = reinterpret_cast<float*>(smem);       // [W][COLS] maxima, sums, then [W][COLS][D]
@@ -1061,20 +1138,17 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const A
   constexpr int NS = SCORE_STAGES, W = SCORE_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float sm[W][Y::COLS], sl[W][Y::COLS];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   const int r = lane / 4, c = lane % 4;
   const int64_t kv = blockIdx.y;
   const int split = blockIdx.x / p.ztiles, col0 = (blockIdx.x % p.ztiles) * Y::COLS;
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
   const Steps sp(p, true);
-  const Source<BITS, G, NG, false> src(p, kv, lane);
   const int first = split * W + warp, stride = p.splits * W;
+  Source<BITS, G, NG, false> src(p, kv, lane, (int64_t)first * 32, (int64_t)stride * 32);
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) {
-    const int u = first + i * stride;
-    if (u < sp.total) src.fetch(p, sp, u, ring + i * S::BYTES, kv, lane);
-    cp_async_commit();
-  }
+  for (int i = 0; i < NS - 1; ++i) src.fetch(p, sp, first + i * stride, ring + i * S::BYTES, kv, lane);
   Query<BITS, G, NG, SPLIT, NT> q;
   q.load(p, kv, col0, lane);
   float m[NT][2], l[NT][2];  // of this thread's keys
@@ -1085,45 +1159,52 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const A
       m[nt][k] = M_NONE;
       l[nt][k] = 0.f;
     }
-  int at = 0;
-  for (int u = first; u < sp.total; u += stride) {
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    const int ahead = u + (NS - 1) * stride;
-    if (ahead < sp.total) src.fetch(p, sp, ahead, ring + (at == 0 ? NS - 1 : at - 1) * S::BYTES, kv, lane);
-    cp_async_commit();
-    const uint32_t st = ring + at * S::BYTES;
-    at = at == NS - 1 ? 0 : at + 1;
+  // This thread's scores in its first step: key row key_of(r), columns 2c, 2c + 1; a step on is `jump` floats on.
+  float* out = p.scores + (kv * p.cap + (int64_t)first * 32 + key_of(r)) * p.gp + col0;
+  const int64_t jump = (int64_t)stride * 32 * p.gp;
+  auto take = [&](uint32_t st, bool whole, int keys) {  // keys: those of the step from this thread's first on
     float s[Y::TILES * NT][4];
     step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
+    bool move = false;
 #pragma unroll
     for (int x = 0; x < Y::TILES; ++x)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float(&v)[4] = s[x * NT + nt];
-        const int pos = u * 32 + Y::tile(x, c) * 16 + key_of(r);
-        const int col = col0 + Y::col(nt, c, 0);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const bool ok = pos + h * 8 < sp.n;
+          const int row = Y::tile(x, c) * 16 + h * 8, col = Y::col(nt, c, 0);
+          const bool ok = whole || row < keys;
 #pragma unroll
           for (int k = 0; k < 2; ++k) v[2 * h + k] = ok ? v[2 * h + k] * q.mul[nt][k] : -INFINITY;
-          if (col < p.gp && ok)
-            *reinterpret_cast<float2*>(p.scores + ((kv * p.cap + pos + h * 8) * p.gp + col)) =
-                make_float2(v[2 * h], v[2 * h + 1]);
+          if (col0 + col < p.gp && ok)
+            *reinterpret_cast<float2*>(out + row * p.gp + col) = make_float2(v[2 * h], v[2 * h + 1]);
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float top = fmaxf(v[k], v[2 + k]);
-          if (top > m[nt][k] + LAZY) {
-            l[nt][k] *= fast_exp2(m[nt][k] - top);
-            m[nt][k] = top;
-          }
-          l[nt][k] += fast_exp2(v[k] - m[nt][k]) + fast_exp2(v[2 + k] - m[nt][k]);
-        }
+        for (int k = 0; k < 2; ++k) move |= fmaxf(v[k], v[2 + k]) > m[nt][k] + LAZY;
       }
-  }
-  cp_async_wait<0>();
+    out += jump;
+    if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float next = m[nt][k];
+#pragma unroll
+          for (int x = 0; x < Y::TILES; ++x) next = fmax3(next, s[x * NT + nt][k], s[x * NT + nt][2 + k]);
+          l[nt][k] *= fast_exp2(m[nt][k] - next);
+          m[nt][k] = next;
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < Y::TILES; ++x)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[nt][i & 1] += fast_exp2(s[x * NT + nt][i] - m[nt][i & 1]);
+  };
+  run_steps<NS>(p, sp, src, ring, first, stride, kv, lane, [&](uint32_t st) { take(st, true, 32); },
+                [&](int u, uint32_t st) { take(st, false, sp.n - u * 32 - key_of(r)); });
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
