@@ -129,6 +129,7 @@ class QkvAttnArgs(C.Structure):
                 ("out_probs", vp),
                 ("out_idx", vp), ("so_i", i64),
                 ("splits", i64),
+                ("tickets", vp), ("n_tickets", i64),
                 ("scale", f32), ("dtype", C.c_int), ("idx_i64", C.c_int), ("out_idx_i64", C.c_int)]
 
 

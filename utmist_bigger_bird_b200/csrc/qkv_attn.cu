@@ -2,8 +2,8 @@
 // (semantics: include/bb_b200.h, bb_qkv_decode and bb_qkv_route).
 //
 //   qkv_partial_kernel  up to 4, 8 or 16 query rows of one KV head over one split of its key list: running max,
-//                       sum and P.V of the split, in fp32
-//   qkv_combine_kernel  merges the splits of a row
+//                       sum and P.V of the split, in fp32; the last CTA of a tile to arrive merges its splits
+//   qkv_combine_kernel  merges them where the caller gave no tickets
 //   qkv_scores_kernel   log2 scores of every key for the query heads of a KV head, and per-split softmax
 //                       statistics
 //   qkv_pool_kernel     merged statistics, probabilities averaged over the query heads of a KV head
@@ -54,8 +54,9 @@ struct AttnParams {
   int d, heads, groups, t, cols, gp, splits, ztiles, dtype;
   int q16;          // query rows on 16-byte boundaries
   float scale_log2;
-  float2* part_ml;  // [heads * t][splits] (max in log2 units, sum); routing: [heads][splits]
-  float* part_acc;  // [heads * t][splits][d]
+  float2* part_ml;  // (max in log2 units, sum): [kv_heads * ztiles][splits][columns]; routing: [heads][splits]
+  float* part_acc;  // [kv_heads * ztiles][splits][columns][d]
+  int32_t* tickets; // [kv_heads * ztiles] arrivals, zero between calls; or null
   void* out; int64_t so_h, so_t;
   float* scores;    // routing: [kv_heads][cap][gp] log2 units
   float* probs;     // [kv_heads][cap]
@@ -579,11 +580,16 @@ constexpr int stages(int warps, int bytes) {
   const int fit = 113 * 1024 / (warps * bytes);
   return fit < 2 ? 2 : (fit > 4 ? 4 : fit);
 }
-template <int BITS, int G, int NG, bool SPLIT, int NT> constexpr size_t partial_smem() {
+// Floats of shared memory that combine() uses.
+template <int COLS, int THREADS> constexpr size_t combine_floats(int64_t splits) {
+  return THREADS * 4 + COLS + (size_t)splits * COLS;
+}
+template <int BITS, int G, int NG, bool SPLIT, int NT> size_t partial_smem(int splits) {
   using S = Stage<BITS, G, NG, true>;
   const size_t ring = (size_t)warps<BITS, SPLIT, NT>() * stages(warps<BITS, SPLIT, NT>(), S::BYTES) * S::BYTES;
   const size_t merge = (size_t)warps<BITS, SPLIT, NT>() * Layout<SPLIT, NT>::COLS * (G * 32 + 2) * 4;
-  return ring > merge ? ring : merge;
+  const size_t last = combine_floats<Layout<SPLIT, NT>::COLS, 32 * warps<BITS, SPLIT, NT>()>(splits) * 4;
+  return std::max({ring, merge, last});
 }
 
 // The softmax of a warp's columns: reference points that move only when a score exceeds them by 2^LAZY or a step
@@ -1010,6 +1016,79 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
   }
 };
 
+__device__ __forceinline__ void put_out(const AttnParams& p, int64_t kv, int col, int dim, float x) {
+  const int64_t at = (kv * p.groups + col % p.groups) * p.so_h + (int64_t)(col / p.groups) * p.so_t + dim;
+  if (p.dtype == BB_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(x);
+  else static_cast<__half*>(p.out)[at] = __float2half_rn(x);
+}
+
+// Merges the splits of one tile of query rows: weights first (a warp a row), then four dimensions of a row a thread,
+// the splits dealt to several threads where there are more threads than that. A row that sees no key (a sum
+// of 0) gives zeros.
+template <int COLS, int D, int THREADS>
+__device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64_t kv, int col0, float* smem) {
+  float4* red = reinterpret_cast<float4*>(smem);  // [THREADS]
+  float* inv = smem + THREADS * 4;                // [COLS]
+  float* wt = inv + COLS;                         // [splits][COLS]
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, splits = p.splits;
+  const float2* ml = p.part_ml + tile * splits * COLS;
+  const int cols = min(COLS, p.cols - col0);
+  for (int col = warp; col < cols; col += THREADS / 32) {
+    float M = M_NONE, L = 0.f;
+    for (int s = lane; s < splits; s += 32) M = fmaxf(M, __ldcg(ml + s * COLS + col).x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    for (int s = lane; s < splits; s += 32) {
+      const float2 v = __ldcg(ml + s * COLS + col);
+      const float e = fast_exp2(v.x - M);  // M_NONE: 0, or 1 with a sum of 0 where no split has a key
+      wt[s * COLS + col] = e;
+      L = fmaf(e, v.y, L);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+    if (lane == 0) inv[col] = L == 0.f ? 0.f : 1.f / L;
+  }
+  __syncthreads();
+  constexpr int ITEMS = COLS * D / 4, PARTS = ITEMS < THREADS ? THREADS / ITEMS : 1;
+  const float4* acc = reinterpret_cast<const float4*>(p.part_acc + tile * splits * COLS * D);
+  for (int i0 = 0; i0 < ITEMS; i0 += THREADS) {
+    const int item = i0 + threadIdx.x % (PARTS > 1 ? ITEMS : THREADS), part = PARTS > 1 ? threadIdx.x / ITEMS : 0;
+    const int col = item / (D / 4);
+    const bool mine = part < PARTS && item < ITEMS && col < cols;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine) {
+#pragma unroll 8
+      for (int s = part; s < splits; s += PARTS) {
+        const float4 v = __ldcg(acc + (int64_t)s * ITEMS + item);
+        const float w = wt[s * COLS + col];
+        a.x = fmaf(w, v.x, a.x);
+        a.y = fmaf(w, v.y, a.y);
+        a.z = fmaf(w, v.z, a.z);
+        a.w = fmaf(w, v.w, a.w);
+      }
+    }
+    if (PARTS > 1) {
+      red[threadIdx.x] = a;
+      __syncthreads();
+      if (mine && part == 0)
+        for (int k = 1; k < PARTS; ++k) {
+          const float4 v = red[k * ITEMS + item];
+          a.x += v.x;
+          a.y += v.y;
+          a.z += v.z;
+          a.w += v.w;
+        }
+    }
+    if (mine && part == 0) {
+      const int dim = item % (D / 4) * 4;
+      put_out(p, kv, col0 + col, dim, a.x * inv[col]);
+      put_out(p, kv, col0 + col, dim + 1, a.y * inv[col]);
+      put_out(p, kv, col0 + col, dim + 2, a.z * inv[col]);
+      put_out(p, kv, col0 + col, dim + 3, a.w * inv[col]);
+    }
+  }
+}
+
 // Grid (splits * ztiles, kv_heads). A warp owns its ring of stages and takes steps split * W + warp, then every
 // (splits * W)-th: no barrier until the warps' results are merged at the end.
 template <int BITS, int G, int NG, bool SPLIT, int NT>
@@ -1064,6 +1143,7 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 2) qkv_partial_
       }
   }
   __syncthreads();
+  const int64_t tile = kv * p.ztiles + blockIdx.x % p.ztiles;
   for (int i = threadIdx.x; i < Y::COLS * D; i += 32 * W) {
     const int col = i / D, dim = i % D;
     if (col0 + col >= p.cols) break;
@@ -1076,58 +1156,34 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 2) qkv_partial_
       L = fmaf(e, sl[w * Y::COLS + col], L);
       A = fmaf(e, so[(w * Y::COLS + col) * D + dim], A);
     }
-    const int64_t row = (kv * p.groups + (col0 + col) % p.groups) * p.t + (col0 + col) / p.groups;
-    const int64_t o_at = row * p.splits + split;
-    if (dim == 0) p.part_ml[o_at] = make_float2(M, L);
-    p.part_acc[o_at * D + dim] = A;
+    if (p.splits == 1) {
+      put_out(p, kv, col0 + col, dim, L == 0.f ? 0.f : A / L);
+    } else {
+      const int64_t at = (tile * p.splits + split) * Y::COLS + col;
+      if (dim == 0) p.part_ml[at] = make_float2(M, L);
+      p.part_acc[at * D + dim] = A;
+    }
   }
+  if (p.splits == 1 || !p.tickets) return;
+  // The last CTA of the tile to arrive merges its splits, always in the same order.
+  __threadfence();
+  __syncthreads();
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    last = atomicAdd(p.tickets + tile, 1) == p.splits - 1;
+    if (last) p.tickets[tile] = 0;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  combine<Y::COLS, D, 32 * W>(p, tile, kv, col0, reinterpret_cast<float*>(smem));
 }
 
-// Grid heads * t; 256 threads: the d dimensions, and 256 / dpad parts of the splits. A row that sees no
-// key (a sum of 0) gives zeros.
-__global__ void __launch_bounds__(256) qkv_combine_kernel(AttnParams p) {
-  __shared__ float red[256];
-  __shared__ float wt[1024];
-  __shared__ float sM[8], sL[8];
-  const int64_t row = blockIdx.x;
-  const float2* ml = p.part_ml + row * p.splits;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  float M = M_NONE;
-  for (int s = threadIdx.x; s < p.splits; s += 256) M = fmaxf(M, ml[s].x);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  if (lane == 0) sM[warp] = M;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) M = fmaxf(M, sM[w]);
-  float L = 0.f;
-  for (int s = threadIdx.x; s < p.splits; s += 256) {
-    const float2 v = ml[s];
-    const float e = fast_exp2(v.x - M);  // M_NONE: 0, or 1 with a sum of 0 where no split has a key
-    wt[s] = e;
-    L = fmaf(e, v.y, L);
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-  if (lane == 0) sL[warp] = L;
-  __syncthreads();
-  L = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) L += sL[w];
-  const int dp = p.d <= 32 ? 32 : (p.d <= 64 ? 64 : 128), parts = 256 / dp;
-  const int dim = threadIdx.x % dp, part = threadIdx.x / dp;
-  float A = 0.f;
-  if (dim < p.d)
-    for (int s = part; s < p.splits; s += parts)
-      if (wt[s] != 0.f) A = fmaf(wt[s], p.part_acc[(row * p.splits + s) * p.d + dim], A);
-  red[threadIdx.x] = A;
-  __syncthreads();
-  if (threadIdx.x >= p.d) return;
-  for (int k = 1; k < parts; ++k) A += red[k * dp + threadIdx.x];
-  const float o = L == 0.f ? 0.f : A / L;
-  const int64_t at = (row / p.t) * p.so_h + (row % p.t) * p.so_t + threadIdx.x;
-  if (p.dtype == BB_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o);
-  else static_cast<__half*>(p.out)[at] = __float2half_rn(o);
+// The same merge as a kernel of its own, for calls without tickets: grid (ztiles, kv_heads).
+template <int COLS, int D> __global__ void __launch_bounds__(256) qkv_combine_kernel(const AttnParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int64_t kv = blockIdx.y;
+  combine<COLS, D, 256>(p, kv * p.ztiles + blockIdx.x, kv, blockIdx.x * COLS, reinterpret_cast<float*>(smem));
 }
 
 // Grid (splits * ztiles, kv_heads): the K half of qkv_partial_kernel; scores go to [kv][key][gp].
@@ -1313,9 +1369,9 @@ int plan_decode(const bb_qkv_attn_args* a, AttnPlan* pl) {
   const int64_t lists = a->route_k > 0 && a->route_rows != a->cache.kv_heads ? a->heads / a->cache.kv_heads : 1;
   if (a->route_k > ((int64_t)1 << 27) / lists) return fail(BB_ERR_UNSUPPORTED, "qkv_decode: too many routed keys");
   plan_grid(a, cdiv(f, (int64_t)32) + cdiv(w, (int64_t)32) + lists * cdiv(a->route_k, (int64_t)32), true, pl);
-  const int64_t rows = a->heads * a->t;
-  pl->ml_bytes = align_up((size_t)(rows * pl->splits) * 8, 256);
-  pl->acc_bytes = align_up((size_t)(rows * pl->splits * a->cache.d) * 4, 256);
+  const int64_t rows = a->cache.kv_heads * pl->ztiles * pl->columns * pl->splits;
+  pl->ml_bytes = align_up((size_t)rows * 8, 256);
+  pl->acc_bytes = align_up((size_t)(rows * a->cache.d) * 4, 256);
   pl->total = pl->ml_bytes + pl->acc_bytes;
   return BB_OK;
 }
@@ -1368,11 +1424,19 @@ template <bool DECODE, int BITS, int G, int NG, bool SPLIT, int NT>
 int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
   const dim3 grid((unsigned)(p.splits * p.ztiles), (unsigned)kv_heads);
   if constexpr (DECODE) {
-    constexpr size_t smem = partial_smem<BITS, G, NG, SPLIT, NT>();
+    const size_t smem = partial_smem<BITS, G, NG, SPLIT, NT>(p.splits);
     auto* kernel = qkv_partial_kernel<BITS, G, NG, SPLIT, NT>;
     if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     kernel<<<grid, 32 * warps<BITS, SPLIT, NT>(), smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_partial_kernel");
+    if (p.splits > 1 && !p.tickets) {
+      constexpr int COLS = Layout<SPLIT, NT>::COLS;
+      const size_t merge = combine_floats<COLS, 256>(p.splits) * 4;
+      auto* after = qkv_combine_kernel<COLS, G * 32>;
+      if (merge > 48 * 1024) cudaFuncSetAttribute(after, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)merge);
+      after<<<dim3((unsigned)p.ztiles, (unsigned)kv_heads), 256, merge, stream>>>(p);
+      BB_CHECK_LAUNCH("qkv_combine_kernel");
+    }
   } else {
     constexpr size_t smem = (size_t)SCORE_WARPS * SCORE_STAGES * Stage<BITS, G, NG, false>::BYTES;
     auto* kernel = qkv_scores_kernel<BITS, G, NG, SPLIT, NT>;
@@ -1431,11 +1495,8 @@ int qkv_decode(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_
     return fail(BB_ERR_WORKSPACE, "qkv_decode: workspace too small (%zu < %zu)", ws_bytes, pl.total);
   if (!a->q || !a->out || (a->route_k > 0 && !a->idx)) return fail(BB_ERR_ARG, "qkv_decode: null pointer");
   AttnParams p = make_params(a, pl, static_cast<char*>(ws));
-  st = launch_attn<true>(a, p, pl.columns, stream);
-  if (st) return st;
-  qkv_combine_kernel<<<(unsigned)(a->heads * a->t), 256, 0, stream>>>(p);
-  BB_CHECK_LAUNCH("qkv_combine_kernel");
-  return BB_OK;
+  if (a->tickets && a->n_tickets >= a->cache.kv_heads * pl.ztiles) p.tickets = a->tickets;
+  return launch_attn<true>(a, p, pl.columns, stream);
 }
 
 int qkv_route_workspace_size(const bb_qkv_attn_args* a, size_t* bytes) {

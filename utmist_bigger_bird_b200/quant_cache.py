@@ -25,6 +25,11 @@ __all__ = ["QuantKV", "quant_decode", "quant_pooled_probs", "quant_route"]
 _HALF = (torch.float16, torch.bfloat16)
 
 
+def _stream(device):
+    """The current stream's handle (``torch.cuda.current_stream`` builds a Stream object for it)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 class QuantKV:
     """Codes and (step, low) pairs of ``kv_heads`` x ``capacity`` rows of keys and of values.
 
@@ -78,8 +83,19 @@ class QuantKV:
             k_codes_h=k_codes.stride(0), k_meta_h=k_meta.stride(0) // 2, v_codes_h=v_codes.stride(0),
             v_meta_h=v_meta.stride(0) // 2, kv_heads=self.kv_heads, cap=self.capacity, d=self.head_dim, bits=bits,
             group=self.group)
-        # Calls fill a copy of this, so that threads may share a cache.
+        # Calls fill copies of these, so that threads may share a cache.
         self._attn = _lib.QkvAttnArgs(cache=self._struct)
+        self._write = _lib.QkvWriteArgs(cache=self._struct)
+        self._read = _lib.QkvReadArgs(cache=self._struct)
+        self._tickets = {}  # of quant_decode, a set a stream: calls on one stream do not overlap
+
+    def _take_tickets(self, stream, need):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(need, dtype=torch.int32, device=self.device)  # zeroed by the graph itself
+        t = self._tickets.get(stream)
+        if t is None or t.numel() < need:
+            t = self._tickets[stream] = torch.zeros(max(need, 1024), dtype=torch.int32, device=self.device)
+        return t
 
     @property
     def nbytes(self):
@@ -92,31 +108,34 @@ class QuantKV:
         as [T, Hkv, d]."""
         if not k.is_cuda or k.device != self.device or v.device != self.device:
             raise ValueError("QuantKV.write requires CUDA tensors on the cache's device")
-        if k.dtype not in _ops._DT or v.dtype != k.dtype:
+        dtype = _ops._DT.get(k.dtype)
+        if dtype is None or v.dtype != k.dtype:
             raise ValueError("QuantKV.write: k and v must share one of f16/bf16/f32")
         if k.ndim != 3 or k.shape != v.shape or k.shape[0] != self.kv_heads or k.shape[2] != self.head_dim:
             raise ValueError("QuantKV.write: k and v must be [Hkv, T, d] of the cache")
         hk, t, d = k.shape
         k, v = _ops.rows_view(k), _ops.rows_view(v)
-        a = _lib.QkvWriteArgs(cache=self._struct, k=k.data_ptr(), sk_h=k.stride(0), sk_t=k.stride(1), v=v.data_ptr(),
-                              sv_h=v.stride(0), sv_t=v.stride(1), t=t, dtype=_ops._DT[k.dtype])
+        a = _lib.QkvWriteArgs.from_buffer_copy(self._write)
+        a.k, a.v, a.t, a.dtype = k.data_ptr(), v.data_ptr(), t, dtype
+        a.sk_h, a.sk_t, _ = k.stride()
+        a.sv_h, a.sv_t, _ = v.stride()
         keep = None
         if isinstance(at, torch.Tensor):
             keep = _ops._n_arg(at, 0, self.device)[2]
             a.at_dev = keep.data_ptr()
         else:
-            a.at = int(at)
-            if a.at < 0 or a.at + t > self.capacity:
-                raise ValueError(f"QuantKV.write: rows [{a.at}, {a.at + t}) outside a cache of {self.capacity}")
+            a.at = at = int(at)
+            if at < 0 or at + t > self.capacity:
+                raise ValueError(f"QuantKV.write: rows [{at}, {at + t}) outside a cache of {self.capacity}")
         out = None
         if values:
             both = torch.empty((2, t, hk, d), dtype=k.dtype, device=self.device)
-            out = both[0].transpose(0, 1), both[1].transpose(0, 1)
-            a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
+            a.out_k = first = both.data_ptr()
+            a.out_v = first + t * hk * d * k.element_size()
             a.sok_h = a.sov_h = d
             a.sok_t = a.sov_t = hk * d
-        _lib.check(_lib.lib().bb_qkv_write(C.byref(a), _ops._stream(k)), "QuantKV.write")
-        del keep
+            out = both.transpose(1, 2).unbind(0)
+        _lib.check(_lib.lib().bb_qkv_write(C.byref(a), _stream(self.device)), "QuantKV.write")
         return out
 
     def read(self, positions=None, *, start=0, stop=None, dtype=torch.bfloat16):
@@ -124,7 +143,8 @@ class QuantKV:
         cache give zeros): (k, v) [Hkv, L, d]."""
         if dtype not in _ops._DT:
             raise ValueError("QuantKV.read: dtype must be one of f16/bf16/f32")
-        a = _lib.QkvReadArgs(cache=self._struct, dtype=_ops._DT[dtype])
+        a = _lib.QkvReadArgs.from_buffer_copy(self._read)
+        a.dtype = _ops._DT[dtype]
         if positions is None:
             stop = self.capacity if stop is None else int(stop)
             if not 0 <= start <= stop <= self.capacity:
@@ -142,14 +162,14 @@ class QuantKV:
             a.sp_h, a.pos_i64 = positions.stride(0), int(positions.dtype == torch.int64)
         hk, d = self.kv_heads, self.head_dim
         both = torch.empty((2, hk, rows, d), dtype=dtype, device=self.device)
-        if not rows:
-            return both[0], both[1]
-        a.rows = rows
-        a.out_k, a.out_v = both.data_ptr(), both[1].data_ptr()
-        a.sok_h = a.sov_h = rows * d
-        a.sok_t = a.sov_t = d
-        _lib.check(_lib.lib().bb_qkv_read(C.byref(a), _ops._stream(self.k_codes)), "QuantKV.read")
-        return both[0], both[1]
+        if rows:
+            a.rows = rows
+            a.out_k = first = both.data_ptr()
+            a.out_v = first + hk * rows * d * both.element_size()
+            a.sok_h = a.sov_h = rows * d
+            a.sok_t = a.sov_t = d
+            _lib.check(_lib.lib().bb_qkv_read(C.byref(a), _stream(self.device)), "QuantKV.read")
+        return both.unbind(0)
 
 
 def _args(q, kv, front, window, scale, n, splits, what):
@@ -204,6 +224,10 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
         out = torch.empty((h, d), dtype=q.dtype, device=q.device)
         a.so_h = d
     a.out = out.data_ptr()
+    stream = _stream(kv.device)
+    need = kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 16)
+    tickets = kv._take_tickets(stream, need)
+    a.tickets, a.n_tickets = tickets.data_ptr(), need
     if indices is not None and indices.shape[-1]:
         if indices.device != q.device or indices.dtype not in (torch.int32, torch.int64):
             raise ValueError("quant_decode: indices must be int32 or int64 on q's device")
@@ -213,17 +237,21 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
             indices = indices.contiguous()
         a.idx, a.si_r, a.route_rows, a.route_k = indices.data_ptr(), indices.stride(0), *indices.shape
         a.idx_i64 = int(indices.dtype == torch.int64)
-    _launch("bb_qkv_decode", a, q, "quant_decode")
+    L = _lib.lib()
+    _launch(L.bb_qkv_decode_workspace_size, L.bb_qkv_decode, a, kv.device, stream, "quant_decode")
     return out if q.ndim == 2 else out.transpose(0, 1)
 
 
-def _launch(name, a, q, what):
+def _launch(size_of, run, a, device, stream, what):
+    size, ref = C.c_size_t(0), C.byref(a)
+    _lib.check(size_of(ref, C.byref(size)), what)
+    ws = torch.empty(size.value, dtype=torch.uint8, device=device)
+    _lib.check(run(ref, ws.data_ptr(), size.value, stream), what)
+
+
+def _route(a, kv, what):
     L = _lib.lib()
-    size = C.c_size_t(0)
-    ref = C.byref(a)
-    _lib.check(getattr(L, name + "_workspace_size")(ref, C.byref(size)), what)
-    ws = torch.empty(size.value, dtype=torch.uint8, device=q.device)
-    _lib.check(getattr(L, name)(ref, ws.data_ptr(), size.value, _ops._stream(q)), what)
+    _launch(L.bb_qkv_route_workspace_size, L.bb_qkv_route, a, kv.device, _stream(kv.device), what)
 
 
 def quant_pooled_probs(q, kv, *, front=64, window=4096, scale=1.0, n=None, splits=None):
@@ -234,7 +262,7 @@ def quant_pooled_probs(q, kv, *, front=64, window=4096, scale=1.0, n=None, split
     a, keep = _args(q, kv, front, window, scale, n, splits, "quant_pooled_probs")
     probs = torch.empty(kv.kv_heads, kv.capacity, dtype=torch.float32, device=kv.device)
     a.out_probs = probs.data_ptr()
-    _launch("bb_qkv_route", a, keep[0], "quant_pooled_probs")
+    _route(a, kv, "quant_pooled_probs")
     return probs
 
 
@@ -251,5 +279,5 @@ def quant_route(q, kv, k_route, *, front=64, window=4096, scale=1.0, n=None, spl
     if not k_route:
         return idx
     a.out_idx, a.so_i, a.route_k, a.out_idx_i64 = idx.data_ptr(), k_route, k_route, 1
-    _launch("bb_qkv_route", a, keep[0], "quant_route")
+    _route(a, kv, "quant_route")
     return idx
