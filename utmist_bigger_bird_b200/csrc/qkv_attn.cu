@@ -573,16 +573,16 @@ template <bool SPLIT, int NT> struct Mask {
   }
 };
 
-// Warps a CTA and stages a warp: two CTAs a SM, with 128 registers a thread for 4 query rows (4 bits), 168 for 8 (and
-// for 8-bit stages, twice as large), 255 for 16.
-template <int BITS, bool SPLIT, int NT> constexpr int warps() { return SPLIT && BITS == 4 ? 8 : (NT == 1 ? 6 : 4); }
+// Warps a CTA and stages a warp: one CTA a SM (so that few partial results are left to merge), with 128 registers a
+// thread for 4 query rows (4 bits), 168 for 8 (and for 8-bit stages, twice as large), 255 for 16.
+template <int BITS, bool SPLIT, int NT> constexpr int warps() { return SPLIT && BITS == 4 ? 16 : (NT == 1 ? 12 : 8); }
 constexpr int stages(int warps, int bytes) {
-  const int fit = 113 * 1024 / (warps * bytes);
+  const int fit = 226 * 1024 / (warps * bytes);
   return fit < 2 ? 2 : (fit > 4 ? 4 : fit);
 }
 // Floats of shared memory that combine() uses.
 template <int COLS, int THREADS> constexpr size_t combine_floats(int64_t splits) {
-  return THREADS * 4 + COLS + (size_t)splits * COLS;
+  return THREADS * 4 + (size_t)splits * COLS;
 }
 template <int BITS, int G, int NG, bool SPLIT, int NT> size_t partial_smem(int splits) {
   using S = Stage<BITS, G, NG, true>;
@@ -1028,25 +1028,35 @@ __device__ __forceinline__ void put_out(const AttnParams& p, int64_t kv, int col
 template <int COLS, int D, int THREADS>
 __device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64_t kv, int col0, float* smem) {
   float4* red = reinterpret_cast<float4*>(smem);  // [THREADS]
-  float* inv = smem + THREADS * 4;                // [COLS]
-  float* wt = inv + COLS;                         // [splits][COLS]
+  float* wt = smem + THREADS * 4;                 // [splits][COLS] weights of the splits in the result
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, splits = p.splits;
   const float2* ml = p.part_ml + tile * splits * COLS;
   const int cols = min(COLS, p.cols - col0);
   for (int col = warp; col < cols; col += THREADS / 32) {
     float M = M_NONE, L = 0.f;
-    for (int s = lane; s < splits; s += 32) M = fmaxf(M, __ldcg(ml + s * COLS + col).x);
+    for (int s0 = 0; s0 < splits; s0 += 64) {  // two splits a lane at a time, kept for their weights
+      float2 v[2];
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    for (int s = lane; s < splits; s += 32) {
-      const float2 v = __ldcg(ml + s * COLS + col);
-      const float e = fast_exp2(v.x - M);  // M_NONE: 0, or 1 with a sum of 0 where no split has a key
-      wt[s * COLS + col] = e;
-      L = fmaf(e, v.y, L);
+      for (int k = 0; k < 2; ++k) {
+        const int s = s0 + k * 32 + lane;
+        v[k] = s < splits ? __ldcg(ml + s * COLS + col) : make_float2(M_NONE, 0.f);
+      }
+      float top = fmax3(M, v[0].x, v[1].x);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      L *= fast_exp2(M - top);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int s = s0 + k * 32 + lane;
+        if (s < splits) wt[s * COLS + col] = v[k].x;
+        L = fmaf(fast_exp2(v[k].x - top), v[k].y, L);  // M_NONE: 0, or 1 with a sum of 0 where no split has a key
+      }
+      M = top;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-    if (lane == 0) inv[col] = L == 0.f ? 0.f : 1.f / L;
+    const float scale = L == 0.f ? 0.f : 1.f / L;
+    for (int s = lane; s < splits; s += 32) wt[s * COLS + col] = fast_exp2(wt[s * COLS + col] - M) * scale;
   }
   __syncthreads();
   constexpr int ITEMS = COLS * D / 4, PARTS = ITEMS < THREADS ? THREADS / ITEMS : 1;
@@ -1081,10 +1091,10 @@ __device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64
     }
     if (mine && part == 0) {
       const int dim = item % (D / 4) * 4;
-      put_out(p, kv, col0 + col, dim, a.x * inv[col]);
-      put_out(p, kv, col0 + col, dim + 1, a.y * inv[col]);
-      put_out(p, kv, col0 + col, dim + 2, a.z * inv[col]);
-      put_out(p, kv, col0 + col, dim + 3, a.w * inv[col]);
+      put_out(p, kv, col0 + col, dim, a.x);
+      put_out(p, kv, col0 + col, dim + 1, a.y);
+      put_out(p, kv, col0 + col, dim + 2, a.z);
+      put_out(p, kv, col0 + col, dim + 3, a.w);
     }
   }
 }
@@ -1092,7 +1102,7 @@ __device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64
 // Grid (splits * ztiles, kv_heads). A warp owns its ring of stages and takes steps split * W + warp, then every
 // (splits * W)-th: no barrier until the warps' results are merged at the end.
 template <int BITS, int G, int NG, bool SPLIT, int NT>
-__global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 2) qkv_partial_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 1) qkv_partial_kernel(const AttnParams p) {
   using S = Stage<BITS, G, NG, true>;
   using Y = Layout<SPLIT, NT>;
   constexpr int NS = stages(warps<BITS, SPLIT, NT>(), S::BYTES), D = G * 32, W = warps<BITS, SPLIT, NT>();
@@ -1144,23 +1154,33 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 2) qkv_partial_
   }
   __syncthreads();
   const int64_t tile = kv * p.ztiles + blockIdx.x % p.ztiles;
+  // Each warp's weight in each query row, and the row's maximum and sum; the maxima become the weights.
+  __shared__ float2 row_ml[Y::COLS];
+  for (int col = warp; col < Y::COLS; col += W) {
+    const float m = lane < W ? sm[lane * Y::COLS + col] : M_NONE;
+    float M = m;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    const float e = fast_exp2(m - M);
+    float L = lane < W ? e * sl[lane * Y::COLS + col] : 0.f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+    if (lane < W) sm[lane * Y::COLS + col] = e;
+    if (lane == 0) row_ml[col] = make_float2(M, L);
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < Y::COLS * D; i += 32 * W) {
     const int col = i / D, dim = i % D;
     if (col0 + col >= p.cols) break;
-    float M = M_NONE, L = 0.f, A = 0.f;
+    float A = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w * Y::COLS + col]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float e = fast_exp2(sm[w * Y::COLS + col] - M);
-      L = fmaf(e, sl[w * Y::COLS + col], L);
-      A = fmaf(e, so[(w * Y::COLS + col) * D + dim], A);
-    }
+    for (int w = 0; w < W; ++w) A = fmaf(sm[w * Y::COLS + col], so[(w * Y::COLS + col) * D + dim], A);
+    const float2 ml = row_ml[col];
     if (p.splits == 1) {
-      put_out(p, kv, col0 + col, dim, L == 0.f ? 0.f : A / L);
+      put_out(p, kv, col0 + col, dim, ml.y == 0.f ? 0.f : A / ml.y);
     } else {
       const int64_t at = (tile * p.splits + split) * Y::COLS + col;
-      if (dim == 0) p.part_ml[at] = make_float2(M, L);
+      if (dim == 0) p.part_ml[at] = ml;
       p.part_acc[at * D + dim] = A;
     }
   }
@@ -1346,14 +1366,14 @@ int check_attn(const bb_qkv_attn_args* a, const char* what, bool need_v) {
   return BB_OK;
 }
 
-// The splits of the key list: enough CTAs for one wave at two a SM, no more than one step of 32 keys a warp. Up to 4
+// The splits of the key list: one wave of CTAs (the scores' kernel runs two a SM, the decode one), no more than one step of 32 keys a warp. Up to 4
 // query rows share products (SPLIT, d = 64 or 128), up to 8 take one column tile, more go 16 at a time.
 void plan_grid(const bb_qkv_attn_args* a, int64_t steps, bool decode, AttnPlan* pl) {
   pl->cols = a->heads / a->cache.kv_heads * a->t;
   pl->columns = pl->cols <= 4 && a->cache.d % 64 == 0 ? 4 : (pl->cols <= 8 ? 8 : 16);
   pl->ztiles = cdiv(pl->cols, (int64_t)pl->columns);
   const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 16 ? warps<4, false, 2>() : (pl->columns == 8 || a->cache.bits == 8 ? warps<8, true, 1>() : warps<4, true, 1>()));
-  const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() * 2 / (a->cache.kv_heads * pl->ztiles));
+  const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() * (decode ? 1 : 2) / (a->cache.kv_heads * pl->ztiles));
   pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(steps, w), (int64_t)1024}));
 }
 
