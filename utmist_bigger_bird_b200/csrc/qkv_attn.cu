@@ -395,26 +395,43 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Query {
   uint32_t f[NT][G][SPLIT ? 4 : 2][2];
   float sum[NT][NG][2], mul[NT][2];
 
-  __device__ __forceinline__ void load(const AttnParams& p, int64_t kv, int col0, int lane) {
+  // The rows as stored: issued before the first keys are asked for, waited for after.
+  struct Raw {
+    uint4 v[NT][G];
+  };
+  static __device__ __forceinline__ void load(Raw& raw, const AttnParams& p, int64_t kv, int col0, int lane) {
     const int r = lane / 4, c = lane % 4;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int col = col0 + (SPLIT ? r & 3 : nt * 8 + r);
       const bool live = col < p.cols;
-      float x[G][8];
-      float top = 0.f;
-      const int64_t at = live ? (kv * p.groups + col % p.groups) * p.sq_h + (int64_t)(col / p.groups) * p.sq_t : 0;
+      const int token = p.t == 1 ? 0 : col / p.groups, head = col - token * p.groups;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (live ? (kv * p.groups + head) * p.sq_h + token * p.sq_t : 0) + c * 8;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        const uint16_t* src = static_cast<const uint16_t*>(p.q) + at + g * 32 + c * 8;
+        raw.v[nt][g] = make_uint4(0u, 0u, 0u, 0u);
         if (live && p.q16) {
-          raw = *reinterpret_cast<const uint4*>(src);
+          raw.v[nt][g] = *reinterpret_cast<const uint4*>(src + g * 32);
         } else if (live) {
-          uint16_t* e = reinterpret_cast<uint16_t*>(&raw);
+          uint16_t e[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = src[i];
+          for (int i = 0; i < 8; ++i) e[i] = src[g * 32 + i];
+          raw.v[nt][g] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                                    e[6] | (uint32_t)e[7] << 16);
         }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void take(const Raw& rows, const AttnParams& p, int lane) {
+    const int r = lane / 4, c = lane % 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[G][8];
+      float top = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint4 raw = rows.v[nt][g];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint32_t w = i < 2 ? raw.x : (i < 4 ? raw.y : (i < 6 ? raw.z : raw.w));
@@ -1029,9 +1046,19 @@ template <int COLS, int D, int THREADS>
 __device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64_t kv, int col0, float* smem) {
   float4* red = reinterpret_cast<float4*>(smem);  // [THREADS]
   float* wt = smem + THREADS * 4;                 // [splits][COLS] weights of the splits in the result
+  constexpr int ITEMS = COLS * D / 4, PARTS = ITEMS < THREADS ? THREADS / ITEMS : 1, EARLY = 8;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, splits = p.splits;
   const float2* ml = p.part_ml + tile * splits * COLS;
+  const float4* acc = reinterpret_cast<const float4*>(p.part_acc + tile * splits * COLS * D);
   const int cols = min(COLS, p.cols - col0);
+  const int item0 = threadIdx.x % (PARTS > 1 ? ITEMS : THREADS), part = PARTS > 1 ? threadIdx.x / ITEMS : 0;
+  // this thread's first partial results, asked for before the weights are known
+  float4 early[EARLY];
+#pragma unroll
+  for (int k = 0; k < EARLY; ++k) {
+    const int s = part + k * PARTS;
+    early[k] = part < PARTS && s < splits && item0 / (D / 4) < cols ? __ldcg(acc + (int64_t)s * ITEMS + item0) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   for (int col = warp; col < cols; col += THREADS / 32) {
     float M = M_NONE, L = 0.f;
     for (int s0 = 0; s0 < splits; s0 += 64) {  // two splits a lane at a time, kept for their weights
@@ -1059,23 +1086,26 @@ __device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64
     for (int s = lane; s < splits; s += 32) wt[s * COLS + col] = fast_exp2(wt[s * COLS + col] - M) * scale;
   }
   __syncthreads();
-  constexpr int ITEMS = COLS * D / 4, PARTS = ITEMS < THREADS ? THREADS / ITEMS : 1;
-  const float4* acc = reinterpret_cast<const float4*>(p.part_acc + tile * splits * COLS * D);
   for (int i0 = 0; i0 < ITEMS; i0 += THREADS) {
-    const int item = i0 + threadIdx.x % (PARTS > 1 ? ITEMS : THREADS), part = PARTS > 1 ? threadIdx.x / ITEMS : 0;
-    const int col = item / (D / 4);
+    const int item = i0 + item0, col = item / (D / 4);
     const bool mine = part < PARTS && item < ITEMS && col < cols;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int s, const float4& v) {
+      const float w = wt[s * COLS + col];
+      a.x = fmaf(w, v.x, a.x);
+      a.y = fmaf(w, v.y, a.y);
+      a.z = fmaf(w, v.z, a.z);
+      a.w = fmaf(w, v.w, a.w);
+    };
     if (mine) {
-#pragma unroll 8
-      for (int s = part; s < splits; s += PARTS) {
-        const float4 v = __ldcg(acc + (int64_t)s * ITEMS + item);
-        const float w = wt[s * COLS + col];
-        a.x = fmaf(w, v.x, a.x);
-        a.y = fmaf(w, v.y, a.y);
-        a.z = fmaf(w, v.z, a.z);
-        a.w = fmaf(w, v.w, a.w);
+      int s = part;
+      if (i0 == 0) {
+#pragma unroll
+        for (int k = 0; k < EARLY; ++k, s += PARTS)
+          if (s < splits) add(s, early[k]);
       }
+#pragma unroll 8
+      for (; s < splits; s += PARTS) add(s, __ldcg(acc + (int64_t)s * ITEMS + item));
     }
     if (PARTS > 1) {
       red[threadIdx.x] = a;
@@ -1114,11 +1144,13 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 1) qkv_partial_
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
   const Steps sp(p, false);
   const int first = split * W + warp, stride = p.splits * W;
+  typename Query<BITS, G, NG, SPLIT, NT>::Raw raw;
+  Query<BITS, G, NG, SPLIT, NT>::load(raw, p, kv, col0, lane);
   Source<BITS, G, NG, true> src(p, kv, lane, sp.bf + (int64_t)first * 32, (int64_t)stride * 32);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) src.fetch(p, sp, first + i * stride, ring + i * S::BYTES, kv, lane);
   Query<BITS, G, NG, SPLIT, NT> q;
-  q.load(p, kv, col0, lane);
+  q.take(raw, p, lane);
   Accum<BITS, G, NG, SPLIT, NT> acc;
   acc.clear(lane);
   int since = 0;
@@ -1222,11 +1254,13 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const A
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
   const Steps sp(p, true);
   const int first = split * W + warp, stride = p.splits * W;
+  typename Query<BITS, G, NG, SPLIT, NT>::Raw raw;
+  Query<BITS, G, NG, SPLIT, NT>::load(raw, p, kv, col0, lane);
   Source<BITS, G, NG, false> src(p, kv, lane, (int64_t)first * 32, (int64_t)stride * 32);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) src.fetch(p, sp, first + i * stride, ring + i * S::BYTES, kv, lane);
   Query<BITS, G, NG, SPLIT, NT> q;
-  q.load(p, kv, col0, lane);
+  q.take(raw, p, lane);
   float m[NT][2], l[NT][2];  // of this thread's keys
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)

@@ -25,6 +25,17 @@ __all__ = ["QuantKV", "quant_decode", "quant_pooled_probs", "quant_route"]
 _HALF = (torch.float16, torch.bfloat16)
 
 
+def _rows(x):
+    """x [heads, rows, d] as the kernels can read it (a copy where they cannot), its address and strides."""
+    sh, st, sd = x.stride()
+    p, es = x.data_ptr(), x.element_size()
+    if sd != 1 or (p | sh * es | st * es) & 15:
+        x = x.contiguous()
+        sh, st, _ = x.stride()
+        p = x.data_ptr()
+    return x, p, sh, st
+
+
 def _stream(device):
     """The current stream's handle (``torch.cuda.current_stream`` builds a Stream object for it)."""
     return torch._C._cuda_getCurrentRawStream(device.index)
@@ -87,15 +98,19 @@ class QuantKV:
         self._attn = _lib.QkvAttnArgs(cache=self._struct)
         self._write = _lib.QkvWriteArgs(cache=self._struct)
         self._read = _lib.QkvReadArgs(cache=self._struct)
-        self._tickets = {}  # of quant_decode, a set a stream: calls on one stream do not overlap
+        # Counters (zero between calls) and workspace of quant_decode, a pair a stream: calls on one stream do not
+        # overlap. Calls under a graph capture get their own, which the graph keeps.
+        self._scratch = {}
 
-    def _take_tickets(self, stream, need):
+    def _take_scratch(self, stream, tickets, nbytes):
         if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(need, dtype=torch.int32, device=self.device)  # zeroed by the graph itself
-        t = self._tickets.get(stream)
-        if t is None or t.numel() < need:
-            t = self._tickets[stream] = torch.zeros(max(need, 1024), dtype=torch.int32, device=self.device)
-        return t
+            return (torch.zeros(tickets, dtype=torch.int32, device=self.device),
+                    torch.empty(nbytes, dtype=torch.uint8, device=self.device))
+        s = self._scratch.get(stream)
+        if s is None or s[0].numel() < tickets or s[1].numel() < nbytes:
+            s = self._scratch[stream] = (torch.zeros(max(tickets, 1024), dtype=torch.int32, device=self.device),
+                                         torch.empty(nbytes, dtype=torch.uint8, device=self.device))
+        return s
 
     @property
     def nbytes(self):
@@ -114,11 +129,10 @@ class QuantKV:
         if k.ndim != 3 or k.shape != v.shape or k.shape[0] != self.kv_heads or k.shape[2] != self.head_dim:
             raise ValueError("QuantKV.write: k and v must be [Hkv, T, d] of the cache")
         hk, t, d = k.shape
-        k, v = _ops.rows_view(k), _ops.rows_view(v)
         a = _lib.QkvWriteArgs.from_buffer_copy(self._write)
-        a.k, a.v, a.t, a.dtype = k.data_ptr(), v.data_ptr(), t, dtype
-        a.sk_h, a.sk_t, _ = k.stride()
-        a.sv_h, a.sv_t, _ = v.stride()
+        k, a.k, a.sk_h, a.sk_t = _rows(k)
+        v, a.v, a.sv_h, a.sv_t = _rows(v)
+        a.t, a.dtype = t, dtype
         keep = None
         if isinstance(at, torch.Tensor):
             keep = _ops._n_arg(at, 0, self.device)[2]
@@ -225,9 +239,6 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
         a.so_h = d
     a.out = out.data_ptr()
     stream = _stream(kv.device)
-    need = kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 16)
-    tickets = kv._take_tickets(stream, need)
-    a.tickets, a.n_tickets = tickets.data_ptr(), need
     if indices is not None and indices.shape[-1]:
         if indices.device != q.device or indices.dtype not in (torch.int32, torch.int64):
             raise ValueError("quant_decode: indices must be int32 or int64 on q's device")
@@ -237,21 +248,20 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
             indices = indices.contiguous()
         a.idx, a.si_r, a.route_rows, a.route_k = indices.data_ptr(), indices.stride(0), *indices.shape
         a.idx_i64 = int(indices.dtype == torch.int64)
-    L = _lib.lib()
-    _launch(L.bb_qkv_decode_workspace_size, L.bb_qkv_decode, a, kv.device, stream, "quant_decode")
+    L, size, ref = _lib.lib(), C.c_size_t(0), C.byref(a)
+    _lib.check(L.bb_qkv_decode_workspace_size(ref, C.byref(size)), "quant_decode")
+    need = kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 16)
+    tickets, ws = kv._take_scratch(stream, need, size.value)
+    a.tickets, a.n_tickets = tickets.data_ptr(), need
+    _lib.check(L.bb_qkv_decode(ref, ws.data_ptr(), size.value, stream), "quant_decode")
     return out if q.ndim == 2 else out.transpose(0, 1)
 
 
-def _launch(size_of, run, a, device, stream, what):
-    size, ref = C.c_size_t(0), C.byref(a)
-    _lib.check(size_of(ref, C.byref(size)), what)
-    ws = torch.empty(size.value, dtype=torch.uint8, device=device)
-    _lib.check(run(ref, ws.data_ptr(), size.value, stream), what)
-
-
 def _route(a, kv, what):
-    L = _lib.lib()
-    _launch(L.bb_qkv_route_workspace_size, L.bb_qkv_route, a, kv.device, _stream(kv.device), what)
+    L, size, ref = _lib.lib(), C.c_size_t(0), C.byref(a)
+    _lib.check(L.bb_qkv_route_workspace_size(ref, C.byref(size)), what)
+    ws = torch.empty(size.value, dtype=torch.uint8, device=kv.device)
+    _lib.check(L.bb_qkv_route(ref, ws.data_ptr(), size.value, _stream(kv.device)), what)
 
 
 def quant_pooled_probs(q, kv, *, front=64, window=4096, scale=1.0, n=None, splits=None):
