@@ -35,7 +35,7 @@ size_t topk_scratch_bytes(int64_t rows, int64_t n, int64_t k);
 
 namespace {
 
-constexpr int SCORE_WARPS = 8, SCORE_STAGES = 3;
+constexpr int SCORE_WARPS = 16, SCORE_STAGES = 3;  // one CTA a SM
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float M_NONE = -1.7e38f;   // running maximum before any key (finite: exp2(-inf - M_NONE) is 0)
 constexpr float LAZY = 4.f;          // the running maximum moves only when a score exceeds it by 2^4
@@ -51,14 +51,15 @@ struct AttnParams {
   int idx64, per_head;
   const int64_t* n_dev;
   int64_t n, cap, front, window;
-  int d, heads, groups, t, cols, gp, splits, ztiles, dtype;
+  int d, heads, groups, t, cols, splits, ztiles, dtype;
   int q16;          // query rows on 16-byte boundaries
   float scale_log2;
   float2* part_ml;  // (max in log2 units, sum): [kv_heads * ztiles][splits][columns]; routing: [heads][splits]
   float* part_acc;  // [kv_heads * ztiles][splits][columns][d]
   int32_t* tickets; // [kv_heads * ztiles] arrivals, zero between calls; or null
   void* out; int64_t so_h, so_t;
-  float* scores;    // routing: [kv_heads][cap][gp] log2 units
+  float4* scores;   // routing: log2 units, [kv_heads][steps][ztiles][score tiles][32 threads]
+  int64_t steps;    // of 32 keys in the whole cache
   float* probs;     // [kv_heads][cap]
 };
 
@@ -1240,7 +1241,7 @@ template <int COLS, int D> __global__ void __launch_bounds__(256) qkv_combine_ke
 
 // Grid (splits * ztiles, kv_heads): the K half of qkv_partial_kernel; scores go to [kv][key][gp].
 template <int BITS, int G, int NG, bool SPLIT, int NT>
-__global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(32 * SCORE_WARPS, 1) qkv_scores_kernel(const AttnParams p) {
   using S = Stage<BITS, G, NG, false>;
   using Y = Layout<SPLIT, NT>;
   constexpr int NS = SCORE_STAGES, W = SCORE_WARPS;
@@ -1250,6 +1251,7 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const A
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
   const int r = lane / 4, c = lane % 4;
   const int64_t kv = blockIdx.y;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int split = blockIdx.x / p.ztiles, col0 = (blockIdx.x % p.ztiles) * Y::COLS;
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
   const Steps sp(p, true);
@@ -1269,27 +1271,27 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const A
       m[nt][k] = M_NONE;
       l[nt][k] = 0.f;
     }
-  // This thread's scores in its first step: key row key_of(r), columns 2c, 2c + 1; a step on is `jump` floats on.
-  float* out = p.scores + (kv * p.cap + (int64_t)first * 32 + key_of(r)) * p.gp + col0;
-  const int64_t jump = (int64_t)stride * 32 * p.gp;
+  // Scores are kept as the threads hold them, four a thread and score tile: [kv][step][ztile][score tile][lane].
+  constexpr int SETS = Y::TILES * NT;
+  const int64_t per_step = (int64_t)p.ztiles * SETS * 32;
+  float4* out = p.scores + (kv * p.steps + first) * per_step + blockIdx.x % p.ztiles * SETS * 32 + lane;
+  const int64_t jump = stride * per_step;
   auto take = [&](uint32_t st, bool whole, int keys) {  // keys: those of the step from this thread's first on
-    float s[Y::TILES * NT][4];
+    float s[SETS][4];
     step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
     bool move = false;
 #pragma unroll
     for (int x = 0; x < Y::TILES; ++x)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float(&v)[4] = s[x * NT + nt];
+        const int y = x * NT + nt;
+        float(&v)[4] = s[y];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = Y::tile(x, c) * 16 + h * 8, col = Y::col(nt, c, 0);
-          const bool ok = whole || row < keys;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) v[2 * h + k] = ok ? v[2 * h + k] * q.mul[nt][k] : -INFINITY;
-          if (col0 + col < p.gp && ok)
-            *reinterpret_cast<float2*>(out + row * p.gp + col) = make_float2(v[2 * h], v[2 * h + 1]);
+        for (int i = 0; i < 4; ++i) {
+          v[i] *= q.mul[nt][i & 1];
+          if (!whole && Y::tile(x, c) * 16 + i / 2 * 8 >= keys) v[i] = -INFINITY;
         }
+        out[y * 32] = make_float4(v[0], v[1], v[2], v[3]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) move |= fmaxf(v[k], v[2 + k]) > m[nt][k] + LAZY;
       }
@@ -1342,43 +1344,87 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) qkv_scores_kernel(const A
   }
 }
 
-// Grid (cdiv(cap, 1024), kv_heads); four positions a thread. The merged statistics of the KV head's query
-// heads come first, a warp a head at a time, into shared memory ([groups] maxima, then 1 / sums).
-__global__ void __launch_bounds__(256) qkv_pool_kernel(AttnParams p) {
-  extern __shared__ float stats[];
-  const int64_t kv = blockIdx.y, n = cache_len(p);
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  for (int h = warp; h < p.groups; h += 8) {
-    const float2* ml = p.part_ml + (kv * p.groups + h) * p.splits;
-    float M = M_NONE, L = 0.f;
-    for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, ml[s].x);
+// Grid (blocks of 8 POOL_STEPS steps, kv_heads): a warp pools steps of 32 keys, whose scores it asks for before the
+// statistics are merged. Starts while qkv_scores_kernel runs and waits for its end.
+constexpr int POOL_STEPS = 4;
+template <bool SPLIT, int NT> __global__ void __launch_bounds__(256) qkv_pool_kernel(const AttnParams p) {
+  using Y = Layout<SPLIT, NT>;
+  constexpr int SETS = Y::TILES * NT;
+  extern __shared__ float2 stats[];  // [ztiles * COLS]: maximum, 1 / (sum * groups)
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
+  const int64_t kv = blockIdx.y;
+  const int u0 = (blockIdx.x * 8 + warp) * POOL_STEPS;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t n = cache_len(p), from = p.front, to = n - p.window;  // pooled keys: [from, to)
+  const float4* in = p.scores + kv * p.steps * p.ztiles * SETS * 32 + lane;
+  const int64_t per_step = (int64_t)p.ztiles * SETS * 32;
+  float4 first[POOL_STEPS][SETS];
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    for (int s = lane; s < p.splits; s += 32) L = fmaf(fast_exp2(ml[s].x - M), ml[s].y, L);
+  for (int i = 0; i < POOL_STEPS; ++i) {
+    const int64_t key = (int64_t)(u0 + i) * 32;
+#pragma unroll
+    for (int y = 0; y < SETS; ++y)
+      if (key < to && key + 32 > from) first[i][y] = in[(u0 + i) * per_step + y * 32];
+  }
+  for (int h = warp; h < p.ztiles * Y::COLS; h += 8) {
+    float M = M_NONE, L = 0.f;
+    const float2* ml = p.part_ml + (kv * p.groups + h) * p.splits;
+    for (int s0 = 0; h < p.groups && s0 < p.splits; s0 += 64) {
+      float2 v[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int s = s0 + k * 32 + lane;
+        v[k] = s < p.splits ? ml[s] : make_float2(M_NONE, 0.f);
+      }
+      float top = fmax3(M, v[0].x, v[1].x);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      L *= fast_exp2(M - top);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) L = fmaf(fast_exp2(v[k].x - top), v[k].y, L);
+      M = top;
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-    if (lane == 0) {
-      stats[h] = M;
-      stats[p.groups + h] = 1.f / (L * (float)p.groups);
-    }
+    if (lane == 0) stats[h] = h < p.groups ? make_float2(M, 1.f / (L * (float)p.groups)) : make_float2(0.f, 0.f);
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t pos = (int64_t)blockIdx.x * 1024 + i * 256 + threadIdx.x;
-    if (pos >= p.cap) return;
-    float sum = -1.f;
-    if (pos >= p.front && pos < n - p.window) {
-      const float* row = p.scores + (kv * p.cap + pos) * p.gp;
-      sum = 0.f;
-      for (int h = 0; h < p.groups; ++h) sum = fmaf(fast_exp2(row[h] - stats[h]), stats[p.groups + h], sum);
+  for (int i = 0; i < POOL_STEPS; ++i) {
+    const int64_t key = (int64_t)(u0 + i) * 32;
+    if (key >= p.cap) return;
+    // Thread c of four with one r ends up with key r (c even) or r + 8 (c odd) of tile c / 2.
+    const int64_t pos = key + (c >> 1) * 16 + (c & 1) * 8 + key_of(r);
+    float sum = 0.f;
+    if (key < to && key + 32 > from) {
+      float part[Y::TILES][2] = {};
+      for (int z = 0; z < p.ztiles; ++z)
+#pragma unroll
+        for (int x = 0; x < Y::TILES; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int y = x * NT + nt;
+            const float4 v = z == 0 ? first[i][y] : in[(u0 + i) * per_step + (z * SETS + y) * 32];
+            const float2 a = stats[z * Y::COLS + Y::col(nt, c, 0)], b = stats[z * Y::COLS + Y::col(nt, c, 1)];
+            part[x][0] = fmaf(fast_exp2(v.x - a.x), a.y, fmaf(fast_exp2(v.y - b.x), b.y, part[x][0]));
+            part[x][1] = fmaf(fast_exp2(v.z - a.x), a.y, fmaf(fast_exp2(v.w - b.x), b.y, part[x][1]));
+          }
+#pragma unroll
+      for (int x = 0; x < Y::TILES; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          part[x][h] += __shfl_xor_sync(0xffffffffu, part[x][h], 1);
+          if (!SPLIT) part[x][h] += __shfl_xor_sync(0xffffffffu, part[x][h], 2);
+        }
+      const float(&own)[2] = part[Y::TILES == 1 ? 0 : c >> 1];
+      sum = c & 1 ? own[1] : own[0];
     }
-    p.probs[kv * p.cap + pos] = sum;
+    if (pos < p.cap) p.probs[kv * p.cap + pos] = pos >= from && pos < to ? sum : -1.f;
   }
 }
 
 struct AttnPlan {
-  int64_t splits, ztiles, cols, gp;
+  int64_t splits, ztiles, cols;
   int columns;  // 4 (SPLIT), 8 or 16 query rows a warp
   size_t ml_bytes, acc_bytes, scores_bytes, probs_bytes, topk_bytes, total;
 };
@@ -1400,14 +1446,14 @@ int check_attn(const bb_qkv_attn_args* a, const char* what, bool need_v) {
   return BB_OK;
 }
 
-// The splits of the key list: one wave of CTAs (the scores' kernel runs two a SM, the decode one), no more than one step of 32 keys a warp. Up to 4
+// The splits of the key list: one wave of CTAs, one a SM, and no more than one step of 32 keys a warp. Up to 4
 // query rows share products (SPLIT, d = 64 or 128), up to 8 take one column tile, more go 16 at a time.
 void plan_grid(const bb_qkv_attn_args* a, int64_t steps, bool decode, AttnPlan* pl) {
   pl->cols = a->heads / a->cache.kv_heads * a->t;
   pl->columns = pl->cols <= 4 && a->cache.d % 64 == 0 ? 4 : (pl->cols <= 8 ? 8 : 16);
   pl->ztiles = cdiv(pl->cols, (int64_t)pl->columns);
   const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 16 ? warps<4, false, 2>() : (pl->columns == 8 || a->cache.bits == 8 ? warps<8, true, 1>() : warps<4, true, 1>()));
-  const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() * (decode ? 1 : 2) / (a->cache.kv_heads * pl->ztiles));
+  const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() / (a->cache.kv_heads * pl->ztiles));
   pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(steps, w), (int64_t)1024}));
 }
 
@@ -1437,9 +1483,9 @@ int plan_route(const bb_qkv_attn_args* a, AttnPlan* pl) {
   if (a->route_k > a->cache.cap) return fail(BB_ERR_ARG, "qkv_route: route_k must lie in [0, capacity]");
   *pl = {};
   plan_grid(a, cdiv(a->n_dev ? a->cache.cap : a->n, (int64_t)32), false, pl);
-  pl->gp = align_up(pl->cols, 2);
   pl->ml_bytes = align_up((size_t)(a->heads * pl->splits) * 8, 256);
-  pl->scores_bytes = align_up((size_t)(a->cache.kv_heads * pl->gp * a->cache.cap) * 4, 256);
+  // a step of 32 keys: 4 (SPLIT), 8 or 16 scores a key and ztile
+  pl->scores_bytes = (size_t)(a->cache.kv_heads * cdiv(a->cache.cap, (int64_t)32) * pl->ztiles * pl->columns) * 128;
   pl->probs_bytes = a->out_probs ? 0 : align_up((size_t)(a->cache.kv_heads * a->cache.cap) * 4, 256);
   pl->topk_bytes = align_up(topk_scratch_bytes(a->cache.kv_heads, a->cache.cap, a->route_k), 256);
   pl->total = pl->ml_bytes + pl->scores_bytes + pl->probs_bytes + pl->topk_bytes;
@@ -1463,12 +1509,13 @@ AttnParams make_params(const bb_qkv_attn_args* a, const AttnPlan& pl, char* ws) 
   p.front = a->front; p.window = a->window;
   p.d = (int)c.d;
   p.heads = (int)a->heads; p.groups = (int)(a->heads / c.kv_heads);
-  p.t = (int)a->t; p.cols = (int)pl.cols; p.gp = (int)pl.gp;
+  p.t = (int)a->t; p.cols = (int)pl.cols;
   p.splits = (int)pl.splits; p.ztiles = (int)pl.ztiles; p.dtype = a->dtype;
   p.scale_log2 = a->scale * LOG2E;
   p.part_ml = reinterpret_cast<float2*>(ws);
   p.part_acc = reinterpret_cast<float*>(ws + pl.ml_bytes);
-  p.scores = reinterpret_cast<float*>(ws + pl.ml_bytes);
+  p.scores = reinterpret_cast<float4*>(ws + pl.ml_bytes);
+  p.steps = cdiv(c.cap, (int64_t)32);
   p.probs = a->out_probs ? a->out_probs : reinterpret_cast<float*>(ws + pl.ml_bytes + pl.scores_bytes);
   p.out = a->out; p.so_h = a->so_h; p.so_t = a->so_t;
   return p;
@@ -1498,6 +1545,23 @@ int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
     kernel<<<grid, 32 * SCORE_WARPS, smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_scores_kernel");
   }
+  return BB_OK;
+}
+
+template <bool SPLIT, int NT> int launch_pool(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)cdiv(p.steps, (int64_t)8 * POOL_STEPS), (unsigned)kv_heads);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = (size_t)p.ztiles * Layout<SPLIT, NT>::COLS * 8;
+  cfg.stream = stream;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, qkv_pool_kernel<SPLIT, NT>, p);
+  if (e != cudaSuccess) return fail(BB_ERR_LAUNCH, "qkv_pool_kernel: %s", cudaGetErrorString(e));
+  BB_CHECK_LAUNCH("qkv_pool_kernel");
   return BB_OK;
 }
 
@@ -1572,9 +1636,10 @@ int qkv_route(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_t
   AttnParams p = make_params(a, pl, w);
   st = launch_attn<false>(a, p, pl.columns, stream);
   if (st) return st;
-  qkv_pool_kernel<<<dim3((unsigned)cdiv(a->cache.cap, (int64_t)1024), (unsigned)a->cache.kv_heads), 256,
-                    (size_t)p.groups * 8, stream>>>(p);
-  BB_CHECK_LAUNCH("qkv_pool_kernel");
+  st = pl.columns == 4 ? launch_pool<true, 1>(p, a->cache.kv_heads, stream)
+                       : (pl.columns == 8 ? launch_pool<false, 1>(p, a->cache.kv_heads, stream)
+                                          : launch_pool<false, 2>(p, a->cache.kv_heads, stream));
+  if (st) return st;
   if (a->route_k > 0 && a->out_idx)
     return topk_sorted(p.probs, a->cache.kv_heads, a->cache.cap, a->route_k, a->out_idx, a->out_idx_i64 != 0, a->so_i,
                        w + pl.ml_bytes + pl.scores_bytes + pl.probs_bytes, pl.topk_bytes, stream);
