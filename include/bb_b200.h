@@ -371,7 +371,7 @@ typedef struct {
   void* out_idx; int64_t so_i;
   int64_t splits;                         /* 0: chosen to fill the GPU */
   int32_t* tickets; int64_t n_tickets;    /* bb_qkv_decode: device counters, all zero when the call runs and left zero;
-                                             with one for every KV head and 16 query rows (H / Hkv * t rows a KV
+                                             with one for every KV head and 8 query rows (H / Hkv * t rows a KV
                                              head) the call takes one launch, else (NULL) two. Calls that may
                                              overlap on the GPU need their own. */
   float scale;

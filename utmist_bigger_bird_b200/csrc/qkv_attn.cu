@@ -376,119 +376,112 @@ __device__ __forceinline__ void mma_sum(float (&d)[4], int half, uint32_t b) {
 //     stand in columns 0-3 against the first tile's dimensions and in columns 4-7 against the second's
 //     (zeros elsewhere). One product gives the scores of 32 keys, and every thread's four scores are
 //     distinct (key, query) pairs, so the softmax costs half as much as with four idle columns.
-//   else: NT column tiles of 8 query rows, the two key tiles one after the other.
-template <bool SPLIT, int NT> struct Layout {
-  static constexpr int COLS = SPLIT ? 4 : 8 * NT;   // query rows of a warp
+//   else: 8 query rows in the columns, the two key tiles one after the other.
+template <bool SPLIT> struct Layout {
+  static constexpr int COLS = SPLIT ? 4 : 8;        // query rows of a warp
   static constexpr int TILES = SPLIT ? 1 : 2;       // score tiles a step
-  static_assert(!SPLIT || NT == 1, "SPLIT has one column tile");
-  // Query row of column 8 nt + 2c + k, and the key tile (of a split step) that it belongs to.
-  static __device__ __forceinline__ int col(int nt, int c, int k) { return SPLIT ? (2 * c + k) & 3 : nt * 8 + 2 * c + k; }
+  // Query row of column 2c + k, and the key tile (of a split step) that it belongs to.
+  static __device__ __forceinline__ int col(int c, int k) { return SPLIT ? (2 * c + k) & 3 : 2 * c + k; }
   static __device__ __forceinline__ int tile(int x, int c) { return SPLIT ? c >> 1 : x; }
 };
 
 // The query side of a warp: operands for its columns (query row = token * groups + head within the KV head's
 // query heads), and, for this thread's columns, the sums of each group's elements and the factor that
 // turns (codes . operand) into a log2 score.
-template <int BITS, int G, int NG, bool SPLIT, int NT> struct Query {
-  using Y = Layout<SPLIT, NT>;
+template <int BITS, int G, int NG, bool SPLIT> struct Query {
+  using Y = Layout<SPLIT>;
   // four sets of dimensions a block of 32, as they come out of a word of codes: SPLIT: a product each; else two
   // products of two sets
-  uint32_t f[NT][G][SPLIT ? 4 : 2][2];
-  float sum[NT][NG][2], mul[NT][2];
+  uint32_t f[G][SPLIT ? 4 : 2][2];
+  float sum[NG][2], mul[2];
 
   // The rows as stored: issued before the first keys are asked for, waited for after.
   struct Raw {
-    uint4 v[NT][G];
+    uint4 v[G];
   };
   static __device__ __forceinline__ void load(Raw& raw, const AttnParams& p, int64_t kv, int col0, int lane) {
     const int r = lane / 4, c = lane % 4;
+    const int col = col0 + (SPLIT ? r & 3 : r);
+    const bool live = col < p.cols;
+    const int token = p.t == 1 ? 0 : col / p.groups, head = col - token * p.groups;
+    const uint16_t* src = static_cast<const uint16_t*>(p.q) + (live ? (kv * p.groups + head) * p.sq_h + token * p.sq_t : 0) + c * 8;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int col = col0 + (SPLIT ? r & 3 : nt * 8 + r);
-      const bool live = col < p.cols;
-      const int token = p.t == 1 ? 0 : col / p.groups, head = col - token * p.groups;
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (live ? (kv * p.groups + head) * p.sq_h + token * p.sq_t : 0) + c * 8;
+    for (int g = 0; g < G; ++g) {
+      raw.v[g] = make_uint4(0u, 0u, 0u, 0u);
+      if (live && p.q16) {
+        raw.v[g] = *reinterpret_cast<const uint4*>(src + g * 32);
+      } else if (live) {
+        uint16_t e[8];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        raw.v[nt][g] = make_uint4(0u, 0u, 0u, 0u);
-        if (live && p.q16) {
-          raw.v[nt][g] = *reinterpret_cast<const uint4*>(src + g * 32);
-        } else if (live) {
-          uint16_t e[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = src[g * 32 + i];
-          raw.v[nt][g] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
-                                    e[6] | (uint32_t)e[7] << 16);
-        }
+        for (int i = 0; i < 8; ++i) e[i] = src[g * 32 + i];
+        raw.v[g] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                                  e[6] | (uint32_t)e[7] << 16);
       }
     }
   }
 
   __device__ __forceinline__ void take(const Raw& rows, const AttnParams& p, int lane) {
     const int r = lane / 4, c = lane % 4;
+    float x[G][8];
+    float top = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float x[G][8];
-      float top = 0.f;
+    for (int g = 0; g < G; ++g) {
+      const uint4 raw = rows.v[g];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint4 raw = rows.v[nt][g];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t w = i < 2 ? raw.x : (i < 4 ? raw.y : (i < 6 ? raw.z : raw.w));
-          const uint16_t h = (uint16_t)(i % 2 ? w >> 16 : w);
-          x[g][i] = p.dtype == BB_BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
-          top = fmaxf(top, fabsf(x[g][i]));
-        }
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = i < 2 ? raw.x : (i < 4 ? raw.y : (i < 6 ? raw.z : raw.w));
+        const uint16_t h = (uint16_t)(i % 2 ? w >> 16 : w);
+        x[g][i] = p.dtype == BB_BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+        top = fmaxf(top, fabsf(x[g][i]));
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^e with top 2^e in [2^10, 2^11)
-      int e = 10 - ((int)((__float_as_uint(top) >> 23) & 255) - 127);
-      e = top == 0.f ? 0 : max(-118, min(118, e));
-      const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
-      float s[NG];
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^e with top 2^e in [2^10, 2^11)
+    int e = 10 - ((int)((__float_as_uint(top) >> 23) & 255) - 127);
+    e = top == 0.f ? 0 : max(-118, min(118, e));
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+    float s[NG];
 #pragma unroll
-      for (int i = 0; i < NG; ++i) s[i] = 0.f;
+    for (int i = 0; i < NG; ++i) s[i] = 0.f;
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
+    for (int g = 0; g < G; ++g) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[g / (G / NG)] += x[g][i];
-        // Sets of dimensions in the order in which codes come out of a word. 4 bits: (0,4) (1,5) (2,6) (3,7), the
-        // even sets at 2^-24 and the odd ones at 2^-20; 8 bits: (0,2) (1,3) (4,6) (5,7), all at 2^-24.
-        uint32_t h[4];
+      for (int i = 0; i < 8; ++i) s[g / (G / NG)] += x[g][i];
+      // Sets of dimensions in the order in which codes come out of a word. 4 bits: (0,4) (1,5) (2,6) (3,7), the
+      // even sets at 2^-24 and the odd ones at 2^-20; 8 bits: (0,2) (1,3) (4,6) (5,7), all at 2^-24.
+      uint32_t h[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i0 = BITS == 4 ? k : (k / 2) * 4 + k % 2, i1 = BITS == 4 ? k + 4 : i0 + 2;
+        const float w = BITS == 4 && k % 2 ? up : up * 16.f;
+        h[k] = pack2<__half>(x[g][i0] * w, x[g][i1] * w);
+      }
+      if constexpr (SPLIT) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int i0 = BITS == 4 ? k : (k / 2) * 4 + k % 2, i1 = BITS == 4 ? k + 4 : i0 + 2;
-          const float w = BITS == 4 && k % 2 ? up : up * 16.f;
-          h[k] = pack2<__half>(x[g][i0] * w, x[g][i1] * w);
+          f[g][k][0] = r < 4 ? h[k] : 0u;
+          f[g][k][1] = r < 4 ? 0u : h[k];
         }
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            f[nt][g][k][0] = r < 4 ? h[k] : 0u;
-            f[nt][g][k][1] = r < 4 ? 0u : h[k];
-          }
-        } else if constexpr (BITS == 4) {
-          f[nt][g][0][0] = h[0]; f[nt][g][0][1] = h[2];
-          f[nt][g][1][0] = h[1]; f[nt][g][1][1] = h[3];
-        } else {
-          f[nt][g][0][0] = h[0]; f[nt][g][0][1] = h[1];
-          f[nt][g][1][0] = h[2]; f[nt][g][1][1] = h[3];
-        }
+      } else if constexpr (BITS == 4) {
+        f[g][0][0] = h[0]; f[g][0][1] = h[2];
+        f[g][1][0] = h[1]; f[g][1][1] = h[3];
+      } else {
+        f[g][0][0] = h[0]; f[g][0][1] = h[1];
+        f[g][1][0] = h[2]; f[g][1][1] = h[3];
       }
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        s[i] += __shfl_xor_sync(0xffffffffu, s[i], 1);
-        s[i] += __shfl_xor_sync(0xffffffffu, s[i], 2);
-        s[i] *= up * 9.5367431640625e-07f;  // 2^-20: in units of the codes' products
-#pragma unroll
-        for (int k = 0; k < 2; ++k) sum[nt][i][k] = __shfl_sync(0xffffffffu, s[i], (2 * c + k) * 4);
-      }
-      const float m = p.scale_log2 * 1048576.f * down;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) mul[nt][k] = __shfl_sync(0xffffffffu, m, (2 * c + k) * 4);
     }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      s[i] += __shfl_xor_sync(0xffffffffu, s[i], 1);
+      s[i] += __shfl_xor_sync(0xffffffffu, s[i], 2);
+      s[i] *= up * 9.5367431640625e-07f;  // 2^-20: in units of the codes' products
+#pragma unroll
+      for (int k = 0; k < 2; ++k) sum[i][k] = __shfl_sync(0xffffffffu, s[i], (2 * c + k) * 4);
+    }
+    const float m = p.scale_log2 * 1048576.f * down;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) mul[k] = __shfl_sync(0xffffffffu, m, (2 * c + k) * 4);
   }
 };
 
@@ -503,12 +496,12 @@ template <int BITS, int N> __device__ __forceinline__ uint32_t code_set(const ui
   }
 }
 
-// Scores of a staged step before the columns' factors: s[x * NT + nt] = (slot r, columns 2c, 2c + 1),
+// Scores of a staged step before the columns' factors: s[x] = (slot r, columns 2c, 2c + 1),
 // (slot r + 8, ...) of key tile Layout::tile(x, c).
-template <int BITS, int G, int NG, bool SPLIT, int NT>
-__device__ __forceinline__ void step_scores(const Query<BITS, G, NG, SPLIT, NT>& q, uint32_t rows, uint32_t meta, int lane,
-                                            float (&s)[Layout<SPLIT, NT>::TILES * NT][4]) {
-  using Y = Layout<SPLIT, NT>;
+template <int BITS, int G, int NG, bool SPLIT>
+__device__ __forceinline__ void step_scores(const Query<BITS, G, NG, SPLIT>& q, uint32_t rows, uint32_t meta, int lane,
+                                            float (&s)[Layout<SPLIT>::TILES][4]) {
+  using Y = Layout<SPLIT>;
   const int r = lane / 4, c = lane % 4;
 #pragma unroll
   for (int x = 0; x < Y::TILES; ++x) {
@@ -519,7 +512,7 @@ __device__ __forceinline__ void step_scores(const Query<BITS, G, NG, SPLIT, NT>&
     lds_words(m1, meta + (Y::tile(x, c) * 16 + r + 8) * NG * 4);
 #pragma unroll
     for (int gi = 0; gi < NG; ++gi) {
-      float acc[NT][4];
+      float acc[4];
 #pragma unroll
       for (int b = 0; b < G / NG; ++b) {
         const int g = gi * (G / NG) + b;
@@ -532,33 +525,27 @@ __device__ __forceinline__ void step_scores(const Query<BITS, G, NG, SPLIT, NT>&
           a[1] = code_set<BITS>(w[1], g, k0);
           a[2] = code_set<BITS>(w[SPLIT ? 2 : 0], g, k1);
           a[3] = code_set<BITS>(w[SPLIT ? 3 : 1], g, k1);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (b == 0 && k == 0) mma_h0(acc[nt], a, q.f[nt][g][k]);
-            else mma_h(acc[nt], a, q.f[nt][g][k]);
-          }
+          if (b == 0 && k == 0) mma_h0(acc, a, q.f[g][k]);
+          else mma_h(acc, a, q.f[g][k]);
         }
       }
       const float s0 = step_of(m0[gi]), l0 = low_of(m0[gi]), s1 = step_of(m1[gi]), l1 = low_of(m1[gi]);
+      float(&o)[4] = s[x];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float(&o)[4] = s[x * NT + nt];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          o[k] = gi == 0 ? l0 * q.sum[nt][gi][k] : fmaf(l0, q.sum[nt][gi][k], o[k]);
-          o[2 + k] = gi == 0 ? l1 * q.sum[nt][gi][k] : fmaf(l1, q.sum[nt][gi][k], o[2 + k]);
-          o[k] = fmaf(s0, acc[nt][k], o[k]);
-          o[2 + k] = fmaf(s1, acc[nt][2 + k], o[2 + k]);
-        }
+      for (int k = 0; k < 2; ++k) {
+        o[k] = gi == 0 ? l0 * q.sum[gi][k] : fmaf(l0, q.sum[gi][k], o[k]);
+        o[2 + k] = gi == 0 ? l1 * q.sum[gi][k] : fmaf(l1, q.sum[gi][k], o[2 + k]);
+        o[k] = fmaf(s0, acc[k], o[k]);
+        o[2 + k] = fmaf(s1, acc[2 + k], o[2 + k]);
       }
     }
   }
 }
 
 // Whether this thread's (key, column) pair i of score tile x counts.
-template <bool SPLIT, int NT> struct Mask {
-  using Y = Layout<SPLIT, NT>;
-  bool ok[Y::TILES * NT][4];
+template <bool SPLIT> struct Mask {
+  using Y = Layout<SPLIT>;
+  bool ok[Y::TILES][4];
   __device__ __forceinline__ void set(const AttnParams& p, const Steps& sp, int u, uint32_t positions, int col0, int lane) {
     const int r = lane / 4, c = lane % 4;
     const bool listed = sp.listed(u);
@@ -578,22 +565,22 @@ template <bool SPLIT, int NT> struct Mask {
           if (pos >= to) pos = -1;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int col = col0 + Y::col(nt, c, k);
-            const int own = sp.n - p.t + col / p.groups;  // the token's own position
-            const bool in_window = pos > own - p.window;
-            const bool list_ok = pos >= p.front && !in_window && (!p.per_head || col % p.groups == list);
-            ok[x * NT + nt][half * 2 + k] = pos >= 0 && pos <= own && (listed ? list_ok : (pos < p.front || in_window));
-          }
+        for (int k = 0; k < 2; ++k) {
+          const int col = col0 + Y::col(c, k);
+          const int own = sp.n - p.t + col / p.groups;  // the token's own position
+          const bool in_window = pos > own - p.window;
+          const bool list_ok = pos >= p.front && !in_window && (!p.per_head || col % p.groups == list);
+          ok[x][half * 2 + k] = pos >= 0 && pos <= own && (listed ? list_ok : (pos < p.front || in_window));
+        }
       }
   }
 };
 
 // Warps a CTA and stages a warp: one CTA a SM (so that few partial results are left to merge), with 128 registers a
-// thread for 4 query rows (4 bits), 168 for 8 (and for 8-bit stages, twice as large), 255 for 16.
-template <int BITS, bool SPLIT, int NT> constexpr int warps() { return SPLIT && BITS == 4 ? 16 : (NT == 1 ? 12 : 8); }
+// thread for 4 query rows in 4 bits, 168 for 8 rows and for 8 bits (whose stages are twice as large). Measured for 64
+// query rows on 32K keys (8 rows at a time): 12 warps 84.6 us, 10: 100, 14: 111, 16: 88; 16 rows at a time with 8 warps
+// of 255 registers: 95.
+template <int BITS, bool SPLIT> constexpr int warps() { return SPLIT && BITS == 4 ? 16 : 12; }
 constexpr int stages(int warps, int bytes) {
   const int fit = 226 * 1024 / (warps * bytes);
   return fit < 2 ? 2 : (fit > 4 ? 4 : fit);
@@ -602,29 +589,27 @@ constexpr int stages(int warps, int bytes) {
 template <int COLS, int THREADS> constexpr size_t combine_floats(int64_t splits) {
   return THREADS * 4 + (size_t)splits * COLS;
 }
-template <int BITS, int G, int NG, bool SPLIT, int NT> size_t partial_smem(int splits) {
+template <int BITS, int G, int NG, bool SPLIT> size_t partial_smem(int splits) {
   using S = Stage<BITS, G, NG, true>;
-  const size_t ring = (size_t)warps<BITS, SPLIT, NT>() * stages(warps<BITS, SPLIT, NT>(), S::BYTES) * S::BYTES;
-  const size_t merge = (size_t)warps<BITS, SPLIT, NT>() * Layout<SPLIT, NT>::COLS * (G * 32 + 2) * 4;
-  const size_t last = combine_floats<Layout<SPLIT, NT>::COLS, 32 * warps<BITS, SPLIT, NT>()>(splits) * 4;
+  const size_t ring = (size_t)warps<BITS, SPLIT>() * stages(warps<BITS, SPLIT>(), S::BYTES) * S::BYTES;
+  const size_t merge = (size_t)warps<BITS, SPLIT>() * Layout<SPLIT>::COLS * (G * 32 + 2) * 4;
+  const size_t last = combine_floats<Layout<SPLIT>::COLS, 32 * warps<BITS, SPLIT>()>(splits) * 4;
   return std::max({ring, merge, last});
 }
 
 // The softmax of a warp's columns: reference points that move only when a score exceeds them by 2^LAZY or a step
 // exceeds its bound, and the sum of p over this thread's keys.
-template <bool SPLIT, int NT> struct Running {
-  using Y = Layout<SPLIT, NT>;
-  float m[NT][2], l[NT][2];
+template <bool SPLIT> struct Running {
+  using Y = Layout<SPLIT>;
+  float m[2], l[2];
   float bound, pscale;  // a power of two above every step so far (2^-100: none); P_SCALE / bound
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        m[nt][k] = M_NONE;
-        l[nt][k] = 0.f;
-      }
+    for (int k = 0; k < 2; ++k) {
+      m[k] = M_NONE;
+      l[k] = 0.f;
+    }
     bound = 7.8886090522101181e-31f;
     pscale = P_SCALE / bound;
   }
@@ -632,23 +617,20 @@ template <bool SPLIT, int NT> struct Running {
   // Scores s (before their factors) -> p in e. Returns whether the references moved: everything kept in units of
   // p is then to be multiplied by f, and P.V by shrink as well.
   template <bool EDGE>
-  __device__ __forceinline__ bool update(float (&e)[Y::TILES * NT][4], const float (&s)[Y::TILES * NT][4],
-                                         const float (&mul)[NT][2], const Mask<SPLIT, NT>& mask, float smax,
-                                         float (&f)[NT][2], float& shrink) {
+  __device__ __forceinline__ bool update(float (&e)[Y::TILES][4], const float (&s)[Y::TILES][4],
+                                         const float (&mul)[2], const Mask<SPLIT>& mask, float smax,
+                                         float (&f)[2], float& shrink) {
     constexpr int X = Y::TILES;
     bool move = smax > bound;
 #pragma unroll
     for (int x = 0; x < X; ++x)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int i = 0; i < 4; ++i) {
+        e[x][i] = fmaf(s[x][i], mul[i & 1], -m[i & 1]);
+        if (EDGE && !mask.ok[x][i]) e[x][i] = -INFINITY;
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int y = x * NT + nt;
-          e[y][i] = fmaf(s[y][i], mul[nt][i & 1], -m[nt][i & 1]);
-          if (EDGE && !mask.ok[y][i]) e[y][i] = -INFINITY;
-        }
-#pragma unroll
-    for (int y = 0; y < X * NT; ++y) move |= fmaxf(fmax3(e[y][0], e[y][1], e[y][2]), e[y][3]) > LAZY;
+    for (int x = 0; x < X; ++x) move |= fmaxf(fmax3(e[x][0], e[x][1], e[x][2]), e[x][3]) > LAZY;
     const bool moved = __any_sync(0xffffffffu, move);
     if (moved) {
       const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)));
@@ -660,51 +642,44 @@ template <bool SPLIT, int NT> struct Running {
         pscale = P_SCALE / next;
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int k = 0; k < 2; ++k) {
+        float v = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float v = -INFINITY;
+        for (int x = 0; x < X; ++x)
 #pragma unroll
-          for (int x = 0; x < X; ++x)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int y = x * NT + nt, i = 2 * h + k;
-              e[y][i] = s[y][i] * mul[nt][k];
-              if (EDGE && !mask.ok[y][i]) e[y][i] = -INFINITY;
-              v = fmaxf(v, e[y][i]);
-            }
-#pragma unroll
-          for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-          const float next = fmaxf(m[nt][k], v);
-          f[nt][k] = fast_exp2(m[nt][k] - next);
-          m[nt][k] = next;
-          l[nt][k] *= f[nt][k];
-#pragma unroll
-          for (int x = 0; x < X; ++x) {
-            e[x * NT + nt][k] -= next;
-            e[x * NT + nt][2 + k] -= next;
+          for (int h = 0; h < 2; ++h) {
+            const int i = 2 * h + k;
+            e[x][i] = s[x][i] * mul[k];
+            if (EDGE && !mask.ok[x][i]) e[x][i] = -INFINITY;
+            v = fmaxf(v, e[x][i]);
           }
+#pragma unroll
+        for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+        const float next = fmaxf(m[k], v);
+        f[k] = fast_exp2(m[k] - next);
+        m[k] = next;
+        l[k] *= f[k];
+#pragma unroll
+        for (int x = 0; x < X; ++x) {
+          e[x][k] -= next;
+          e[x][2 + k] -= next;
         }
+      }
     }
 #pragma unroll
-    for (int x = 0; x < X; ++x)
+    for (int x = 0; x < X; ++x) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int y = x * NT + nt;
+      for (int i = 0; i < 4; ++i) e[x][i] = fast_exp2(e[x][i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[y][i] = fast_exp2(e[y][i]);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) l[nt][k] += e[y][k] + e[y][2 + k];
-      }
+      for (int k = 0; k < 2; ++k) l[k] += e[x][k] + e[x][2 + k];
+    }
     return moved;
   }
   __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], off);
+      for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) l[k] += __shfl_xor_sync(0xffffffffu, l[k], off);
   }
 };
 
@@ -720,37 +695,34 @@ template <int BITS> __device__ __forceinline__ constexpr float code_unit(int t) 
   return BITS == 4 && t == 1 ? 9.5367431640625e-07f : 5.9604644775390625e-08f;
 }
 
-// Up to 8 NT query rows in columns; a product covers 16 keys and 16 dimensions.
-template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
-  using Y = Layout<SPLIT, NT>;
+// Up to 8 query rows in columns; a product covers 16 keys and 16 dimensions.
+template <int BITS, int G, int NG, bool SPLIT> struct Accum {
+  using Y = Layout<SPLIT>;
   using S = Stage<BITS, G, NG, true>;
   static constexpr int VW = (G * BITS + 7) / 8;
-  float o[NT][G][2][4];            // block of 32 dimensions, tile of 16
-  float ps[NT][(NG + 1) / 2][4];   // sum P of groups 2i (rows 0-7) and 2i + 1 (rows 8-15)
-  float mid[NT][NG][2];            // sum p (low + C step) of this thread's keys
-  Running<SPLIT, NT> run;
+  float o[G][2][4];            // block of 32 dimensions, tile of 16
+  float ps[(NG + 1) / 2][4];   // sum P of groups 2i (rows 0-7) and 2i + 1 (rows 8-15)
+  float mid[NG][2];            // sum p (low + C step) of this thread's keys
+  Running<SPLIT> run;
 
   __device__ __forceinline__ void clear(int) {
     run.clear();
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+      for (int i = 0; i < 8; ++i) o[g][i / 4][i % 4] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] = 0.f;
+    for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[i / 4][i % 4] = 0.f;
 #pragma unroll
-      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NG * 2; ++i) mid[nt][i / 2][i % 2] = 0.f;
-    }
+    for (int i = 0; i < NG * 2; ++i) mid[i / 2][i % 2] = 0.f;
   }
 
   template <bool EDGE>
-  __device__ __forceinline__ void step(const Query<BITS, G, NG, SPLIT, NT>& q, uint32_t st, int lane,
-                                       const Mask<SPLIT, NT>& mask) {
+  __device__ __forceinline__ void step(const Query<BITS, G, NG, SPLIT>& q, uint32_t st, int lane,
+                                       const Mask<SPLIT>& mask) {
     const int r = lane / 4, c = lane % 4;
-    float s[2 * NT][4], e[2 * NT][4], f[NT][2], shrink;
-    step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
+    float s[2][4], e[2][4], f[2], shrink;
+    step_scores<BITS, G, NG, SPLIT>(q, st, st + S::KM, lane, s);
     uint32_t m0[2][NG], m1[2][NG];
     float smax = 0.f;
 #pragma unroll
@@ -762,18 +734,15 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
     }
     if (run.template update<EDGE>(e, s, q.mul, mask, smax, f, shrink)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int i = 0; i < NG * 2; ++i) mid[i / 2][i % 2] *= f[i % 2];
 #pragma unroll
-        for (int i = 0; i < NG * 2; ++i) mid[nt][i / 2][i % 2] *= f[nt][i % 2];
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int i = 0; i < 8; ++i) o[g][i / 4][i % 4] *= f[i & 1] * shrink;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[nt][g][i / 4][i % 4] *= f[nt][i & 1] * shrink;
-#pragma unroll
-        for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] *= f[nt][i & 1] * shrink;
-      }
+      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[i / 4][i % 4] *= f[i & 1] * shrink;
     }
-    uint32_t b[NG][2 * NT][2];
+    uint32_t b[NG][2][2];
 #pragma unroll
     for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
@@ -781,28 +750,24 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
         const float s0 = step_of(m0[x][gi]), s1 = step_of(m1[x][gi]);
         const float h0 = fmaf(CENTRE<BITS>, s0, low_of(m0[x][gi])), h1 = fmaf(CENTRE<BITS>, s1, low_of(m1[x][gi]));
         const float t0 = s0 * run.pscale, t1 = s1 * run.pscale;
+        float u[4] = {e[x][0] * t0, e[x][1] * t0, e[x][2] * t1, e[x][3] * t1};
+        if constexpr (EDGE) {  // rows that do not count may hold NaN
+          float z[4] = {e[x][0] * h0, e[x][1] * h0, e[x][2] * h1, e[x][3] * h1};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int y = x * NT + nt;
-          float u[4] = {e[y][0] * t0, e[y][1] * t0, e[y][2] * t1, e[y][3] * t1};
-          if constexpr (EDGE) {  // rows that do not count may hold NaN
-            float z[4] = {e[y][0] * h0, e[y][1] * h0, e[y][2] * h1, e[y][3] * h1};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              u[i] = mask.ok[y][i] ? u[i] : 0.f;
-              z[i] = mask.ok[y][i] ? z[i] : 0.f;
-            }
-            mid[nt][gi][0] += z[0] + z[2];
-            mid[nt][gi][1] += z[1] + z[3];
-          } else {
-            mid[nt][gi][0] = fmaf(e[y][0], h0, fmaf(e[y][2], h1, mid[nt][gi][0]));
-            mid[nt][gi][1] = fmaf(e[y][1], h0, fmaf(e[y][3], h1, mid[nt][gi][1]));
+          for (int i = 0; i < 4; ++i) {
+            u[i] = mask.ok[x][i] ? u[i] : 0.f;
+            z[i] = mask.ok[x][i] ? z[i] : 0.f;
           }
-          b[gi][y][0] = transpose8(pack2<__half>(u[0], u[1]));
-          b[gi][y][1] = transpose8(pack2<__half>(u[2], u[3]));
-          mma_sum(ps[nt][gi / 2], gi % 2, b[gi][y][0]);
-          mma_sum(ps[nt][gi / 2], gi % 2, b[gi][y][1]);
+          mid[gi][0] += z[0] + z[2];
+          mid[gi][1] += z[1] + z[3];
+        } else {
+          mid[gi][0] = fmaf(e[x][0], h0, fmaf(e[x][2], h1, mid[gi][0]));
+          mid[gi][1] = fmaf(e[x][1], h0, fmaf(e[x][3], h1, mid[gi][1]));
         }
+        b[gi][x][0] = transpose8(pack2<__half>(u[0], u[1]));
+        b[gi][x][1] = transpose8(pack2<__half>(u[2], u[3]));
+        mma_sum(ps[gi / 2], gi % 2, b[gi][x][0]);
+        mma_sum(ps[gi / 2], gi % 2, b[gi][x][1]);
       }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -813,11 +778,8 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
       for (int g = 0; g < G; ++g) {
         uint32_t a[2][4];
         operands(a, w, g);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_h(o[nt][g][0], a[0], b[g / (G / NG)][x * NT + nt]);
-          mma_h(o[nt][g][1], a[1], b[g / (G / NG)][x * NT + nt]);
-        }
+        mma_h(o[g][0], a[0], b[g / (G / NG)][x]);
+        mma_h(o[g][1], a[1], b[g / (G / NG)][x]);
       }
     }
   }
@@ -843,17 +805,14 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
 
   __device__ __forceinline__ void settle() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+      for (int i = 0; i < 8; ++i) {
+        const int gi = g / (G / NG);
+        o[g][i / 4][i % 4] = fmaf(-CENTRE<BITS> * code_unit<BITS>(i / 4), ps[gi / 2][gi % 2 * 2 + i % 2], o[g][i / 4][i % 4]);
+      }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int gi = g / (G / NG);
-          o[nt][g][i / 4][i % 4] = fmaf(-CENTRE<BITS> * code_unit<BITS>(i / 4), ps[nt][gi / 2][gi % 2 * 2 + i % 2], o[nt][g][i / 4][i % 4]);
-        }
-#pragma unroll
-      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[nt][i / 4][i % 4] = 0.f;
-    }
+    for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[i / 4][i % 4] = 0.f;
   }
 
   // Adds up over the threads that share a column, and hands every sum of this thread to put(query row, dimension).
@@ -862,22 +821,20 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
     run.finish();
     const int r = lane / 4, c = lane % 4;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi)
+        for (int off = 4; off < 32; off *= 2) mid[gi][k] += __shfl_xor_sync(0xffffffffu, mid[gi][k], off);
 #pragma unroll
-          for (int off = 4; off < 32; off *= 2) mid[nt][gi][k] += __shfl_xor_sync(0xffffffffu, mid[nt][gi][k], off);
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)  // 4 bits: tile t holds dimensions 4r + t, 4r + t + 2; 8 bits: 4r + 2t, + 1
-              put(Y::col(nt, c, k), g * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
-                  fmaf(o[nt][g][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound, mid[nt][g / (G / NG)][k]));
-      }
+          for (int h = 0; h < 2; ++h)  // 4 bits: tile t holds dimensions 4r + t, 4r + t + 2; 8 bits: 4r + 2t, + 1
+            put(Y::col(c, k), g * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
+                fmaf(o[g][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound, mid[g / (G / NG)][k]));
+    }
   }
 };
 
@@ -885,8 +842,8 @@ template <int BITS, int G, int NG, bool SPLIT, int NT> struct Accum {
 // 16-bit operands that comes out of a word of codes holds a dimension of block 2i and one of block 2i + 1 (of
 // one key), the query rows stand in columns 0-3 for the first and in columns 4-7 for the second (zeros
 // elsewhere). All eight columns carry results, half as many accumulators as with idle ones.
-template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
-  using Y = Layout<true, 1>;
+template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true> {
+  using Y = Layout<true>;
   using S = Stage<BITS, G, NG, true>;
   static constexpr int VW = (G * BITS + 7) / 8, PAIRS = G / 2;
   static constexpr int NU = NG < PAIRS ? NG : PAIRS;  // groups that this thread's columns meet
@@ -894,7 +851,7 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
   float o[PAIRS][2][4];
   float ps[4];                     // sum P of this thread's groups 0 (rows 0-7) and 1 (rows 8-15)
   float mid[NU][2];
-  Running<true, 1> run;
+  Running<true> run;
   uint32_t sel0, sel1;             // place the first / second 16 bits of a word in this column's half
 
   __device__ __forceinline__ void clear(int lane) {
@@ -910,10 +867,10 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
   }
 
   template <bool EDGE>
-  __device__ __forceinline__ void step(const Query<BITS, G, NG, true, 1>& q, uint32_t st, int lane, const Mask<true, 1>& mask) {
+  __device__ __forceinline__ void step(const Query<BITS, G, NG, true>& q, uint32_t st, int lane, const Mask<true>& mask) {
     const int r = lane / 4, c = lane % 4;
-    float s[1][4], e[1][4], f[1][2], shrink;
-    step_scores<BITS, G, NG, true, 1>(q, st, st + S::KM, lane, s);
+    float s[1][4], e[1][4], f[2], shrink;
+    step_scores<BITS, G, NG, true>(q, st, st + S::KM, lane, s);
     // (step, low) of this thread's groups: rows r and r + 8 of both tiles
     uint32_t m[4][NU];
     float smax = 0.f;
@@ -931,11 +888,11 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
     }
     if (run.template update<EDGE>(e, s, q.mul, mask, smax, f, shrink)) {
 #pragma unroll
-      for (int i = 0; i < NU * 2; ++i) mid[i / 2][i % 2] *= f[0][i % 2];
+      for (int i = 0; i < NU * 2; ++i) mid[i / 2][i % 2] *= f[i % 2];
 #pragma unroll
-      for (int i = 0; i < PAIRS * 8; ++i) o[i / 8][i / 4 % 2][i % 4] *= f[0][i & 1] * shrink;
+      for (int i = 0; i < PAIRS * 8; ++i) o[i / 8][i / 4 % 2][i % 4] *= f[i & 1] * shrink;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ps[i] *= f[0][i & 1] * shrink;
+      for (int i = 0; i < 4; ++i) ps[i] *= f[i & 1] * shrink;
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -1028,7 +985,7 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true, 1> {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            put(Y::col(0, c, k), (2 * i + (c >> 1)) * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
+            put(Y::col(c, k), (2 * i + (c >> 1)) * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
                 fmaf(o[i][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound, mid[NU == PAIRS ? i : 0][k]));
     }
   }
@@ -1132,11 +1089,11 @@ __device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64
 
 // Grid (splits * ztiles, kv_heads). A warp owns its ring of stages and takes steps split * W + warp, then every
 // (splits * W)-th: no barrier until the warps' results are merged at the end.
-template <int BITS, int G, int NG, bool SPLIT, int NT>
-__global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 1) qkv_partial_kernel(const AttnParams p) {
+template <int BITS, int G, int NG, bool SPLIT>
+__global__ void __launch_bounds__(32 * warps<BITS, SPLIT>(), 1) qkv_partial_kernel(const AttnParams p) {
   using S = Stage<BITS, G, NG, true>;
-  using Y = Layout<SPLIT, NT>;
-  constexpr int NS = stages(warps<BITS, SPLIT, NT>(), S::BYTES), D = G * 32, W = warps<BITS, SPLIT, NT>();
+  using Y = Layout<SPLIT>;
+  constexpr int NS = stages(warps<BITS, SPLIT>(), S::BYTES), D = G * 32, W = warps<BITS, SPLIT>();
   extern __shared__ __align__(128) unsigned char smem[];
   const int lane = threadIdx.x % 32;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);  // known to be the same in all lanes
@@ -1145,27 +1102,27 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 1) qkv_partial_
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
   const Steps sp(p, false);
   const int first = split * W + warp, stride = p.splits * W;
-  typename Query<BITS, G, NG, SPLIT, NT>::Raw raw;
-  Query<BITS, G, NG, SPLIT, NT>::load(raw, p, kv, col0, lane);
+  typename Query<BITS, G, NG, SPLIT>::Raw raw;
+  Query<BITS, G, NG, SPLIT>::load(raw, p, kv, col0, lane);
   Source<BITS, G, NG, true> src(p, kv, lane, sp.bf + (int64_t)first * 32, (int64_t)stride * 32);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) src.fetch(p, sp, first + i * stride, ring + i * S::BYTES, kv, lane);
-  Query<BITS, G, NG, SPLIT, NT> q;
+  Query<BITS, G, NG, SPLIT> q;
   q.take(raw, p, lane);
-  Accum<BITS, G, NG, SPLIT, NT> acc;
+  Accum<BITS, G, NG, SPLIT> acc;
   acc.clear(lane);
   int since = 0;
   run_steps<NS>(
       p, sp, src, ring, first, stride, kv, lane,
       [&](uint32_t st) {
-        acc.template step<false>(q, st, lane, Mask<SPLIT, NT>());
+        acc.template step<false>(q, st, lane, Mask<SPLIT>());
         if (++since == SETTLE) {
           acc.settle();
           since = 0;
         }
       },
       [&](int u, uint32_t st) {
-        Mask<SPLIT, NT> mask;
+        Mask<SPLIT> mask;
         mask.set(p, sp, u, st + S::POS, col0, lane);
         acc.template step<true>(q, st, lane, mask);
         acc.settle();
@@ -1178,12 +1135,10 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT, NT>(), 1) qkv_partial_
   acc.finish(lane, [&](int row, int dim, float x) { so[(warp * Y::COLS + row) * D + dim] = x; });
   if (lane < (SPLIT ? 2 : 4)) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        sm[warp * Y::COLS + Y::col(nt, lane, k)] = acc.run.m[nt][k];
-        sl[warp * Y::COLS + Y::col(nt, lane, k)] = acc.run.l[nt][k];
-      }
+    for (int k = 0; k < 2; ++k) {
+      sm[warp * Y::COLS + Y::col(lane, k)] = acc.run.m[k];
+      sl[warp * Y::COLS + Y::col(lane, k)] = acc.run.l[k];
+    }
   }
   __syncthreads();
   const int64_t tile = kv * p.ztiles + blockIdx.x % p.ztiles;
@@ -1240,10 +1195,10 @@ template <int COLS, int D> __global__ void __launch_bounds__(256) qkv_combine_ke
 }
 
 // Grid (splits * ztiles, kv_heads): the K half of qkv_partial_kernel; scores go to [kv][key][gp].
-template <int BITS, int G, int NG, bool SPLIT, int NT>
+template <int BITS, int G, int NG, bool SPLIT>
 __global__ void __launch_bounds__(32 * SCORE_WARPS, 1) qkv_scores_kernel(const AttnParams p) {
   using S = Stage<BITS, G, NG, false>;
-  using Y = Layout<SPLIT, NT>;
+  using Y = Layout<SPLIT>;
   constexpr int NS = SCORE_STAGES, W = SCORE_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float sm[W][Y::COLS], sl[W][Y::COLS];
@@ -1256,82 +1211,71 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 1) qkv_scores_kernel(const A
   const uint32_t ring = smem_u32(smem) + warp * NS * S::BYTES;
   const Steps sp(p, true);
   const int first = split * W + warp, stride = p.splits * W;
-  typename Query<BITS, G, NG, SPLIT, NT>::Raw raw;
-  Query<BITS, G, NG, SPLIT, NT>::load(raw, p, kv, col0, lane);
+  typename Query<BITS, G, NG, SPLIT>::Raw raw;
+  Query<BITS, G, NG, SPLIT>::load(raw, p, kv, col0, lane);
   Source<BITS, G, NG, false> src(p, kv, lane, (int64_t)first * 32, (int64_t)stride * 32);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) src.fetch(p, sp, first + i * stride, ring + i * S::BYTES, kv, lane);
-  Query<BITS, G, NG, SPLIT, NT> q;
+  Query<BITS, G, NG, SPLIT> q;
   q.take(raw, p, lane);
-  float m[NT][2], l[NT][2];  // of this thread's keys
+  float m[2], l[2];  // of this thread's keys
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      m[nt][k] = M_NONE;
-      l[nt][k] = 0.f;
-    }
+  for (int k = 0; k < 2; ++k) {
+    m[k] = M_NONE;
+    l[k] = 0.f;
+  }
   // Scores are kept as the threads hold them, four a thread and score tile: [kv][step][ztile][score tile][lane].
-  constexpr int SETS = Y::TILES * NT;
+  constexpr int SETS = Y::TILES;
   const int64_t per_step = (int64_t)p.ztiles * SETS * 32;
   float4* out = p.scores + (kv * p.steps + first) * per_step + blockIdx.x % p.ztiles * SETS * 32 + lane;
   const int64_t jump = stride * per_step;
   auto take = [&](uint32_t st, bool whole, int keys) {  // keys: those of the step from this thread's first on
     float s[SETS][4];
-    step_scores<BITS, G, NG, SPLIT, NT>(q, st, st + S::KM, lane, s);
+    step_scores<BITS, G, NG, SPLIT>(q, st, st + S::KM, lane, s);
     bool move = false;
 #pragma unroll
-    for (int x = 0; x < Y::TILES; ++x)
+    for (int x = 0; x < Y::TILES; ++x) {
+      float(&v)[4] = s[x];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int y = x * NT + nt;
-        float(&v)[4] = s[y];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] *= q.mul[nt][i & 1];
-          if (!whole && Y::tile(x, c) * 16 + i / 2 * 8 >= keys) v[i] = -INFINITY;
-        }
-        out[y * 32] = make_float4(v[0], v[1], v[2], v[3]);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) move |= fmaxf(v[k], v[2 + k]) > m[nt][k] + LAZY;
+      for (int i = 0; i < 4; ++i) {
+        v[i] *= q.mul[i & 1];
+        if (!whole && Y::tile(x, c) * 16 + i / 2 * 8 >= keys) v[i] = -INFINITY;
       }
+      out[x * 32] = make_float4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) move |= fmaxf(v[k], v[2 + k]) > m[k] + LAZY;
+    }
     out += jump;
     if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int k = 0; k < 2; ++k) {
+        float next = m[k];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float next = m[nt][k];
-#pragma unroll
-          for (int x = 0; x < Y::TILES; ++x) next = fmax3(next, s[x * NT + nt][k], s[x * NT + nt][2 + k]);
-          l[nt][k] *= fast_exp2(m[nt][k] - next);
-          m[nt][k] = next;
-        }
+        for (int x = 0; x < Y::TILES; ++x) next = fmax3(next, s[x][k], s[x][2 + k]);
+        l[k] *= fast_exp2(m[k] - next);
+        m[k] = next;
+      }
     }
 #pragma unroll
     for (int x = 0; x < Y::TILES; ++x)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l[nt][i & 1] += fast_exp2(s[x * NT + nt][i] - m[nt][i & 1]);
+      for (int i = 0; i < 4; ++i) l[i & 1] += fast_exp2(s[x][i] - m[i & 1]);
   };
   run_steps<NS>(p, sp, src, ring, first, stride, kv, lane, [&](uint32_t st) { take(st, true, 32); },
                 [&](int u, uint32_t st) { take(st, false, sp.n - u * 32 - key_of(r)); });
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int k = 0; k < 2; ++k) {
+    float M = m[k];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float M = m[nt][k];
+    for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    float L = l[k] * fast_exp2(m[k] - M);
 #pragma unroll
-      for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-      float L = l[nt][k] * fast_exp2(m[nt][k] - M);
-#pragma unroll
-      for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) L += __shfl_xor_sync(0xffffffffu, L, off);
-      if (r == 0 && (!SPLIT || c < 2)) {
-        sm[warp][Y::col(nt, c, k)] = M;
-        sl[warp][Y::col(nt, c, k)] = L;
-      }
+    for (int off = SPLIT ? 2 : 4; off < 32; off *= 2) L += __shfl_xor_sync(0xffffffffu, L, off);
+    if (r == 0 && (!SPLIT || c < 2)) {
+      sm[warp][Y::col(c, k)] = M;
+      sl[warp][Y::col(c, k)] = L;
     }
+  }
   __syncthreads();
   const int col = threadIdx.x;
   if (col < Y::COLS && col0 + col < p.cols) {
@@ -1347,9 +1291,9 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 1) qkv_scores_kernel(const A
 // Grid (blocks of 8 POOL_STEPS steps, kv_heads): a warp pools steps of 32 keys, whose scores it asks for before the
 // statistics are merged. Starts while qkv_scores_kernel runs and waits for its end.
 constexpr int POOL_STEPS = 4;
-template <bool SPLIT, int NT> __global__ void __launch_bounds__(256) qkv_pool_kernel(const AttnParams p) {
-  using Y = Layout<SPLIT, NT>;
-  constexpr int SETS = Y::TILES * NT;
+template <bool SPLIT> __global__ void __launch_bounds__(256) qkv_pool_kernel(const AttnParams p) {
+  using Y = Layout<SPLIT>;
+  constexpr int SETS = Y::TILES;
   extern __shared__ float2 stats[];  // [ztiles * COLS]: maximum, 1 / (sum * groups)
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
   const int64_t kv = blockIdx.y;
@@ -1400,15 +1344,12 @@ template <bool SPLIT, int NT> __global__ void __launch_bounds__(256) qkv_pool_ke
       float part[Y::TILES][2] = {};
       for (int z = 0; z < p.ztiles; ++z)
 #pragma unroll
-        for (int x = 0; x < Y::TILES; ++x)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int y = x * NT + nt;
-            const float4 v = z == 0 ? first[i][y] : in[(u0 + i) * per_step + (z * SETS + y) * 32];
-            const float2 a = stats[z * Y::COLS + Y::col(nt, c, 0)], b = stats[z * Y::COLS + Y::col(nt, c, 1)];
-            part[x][0] = fmaf(fast_exp2(v.x - a.x), a.y, fmaf(fast_exp2(v.y - b.x), b.y, part[x][0]));
-            part[x][1] = fmaf(fast_exp2(v.z - a.x), a.y, fmaf(fast_exp2(v.w - b.x), b.y, part[x][1]));
-          }
+        for (int x = 0; x < Y::TILES; ++x) {
+          const float4 v = z == 0 ? first[i][x] : in[(u0 + i) * per_step + (z * SETS + x) * 32];
+          const float2 a = stats[z * Y::COLS + Y::col(c, 0)], b = stats[z * Y::COLS + Y::col(c, 1)];
+          part[x][0] = fmaf(fast_exp2(v.x - a.x), a.y, fmaf(fast_exp2(v.y - b.x), b.y, part[x][0]));
+          part[x][1] = fmaf(fast_exp2(v.z - a.x), a.y, fmaf(fast_exp2(v.w - b.x), b.y, part[x][1]));
+        }
 #pragma unroll
       for (int x = 0; x < Y::TILES; ++x)
 #pragma unroll
@@ -1425,7 +1366,7 @@ template <bool SPLIT, int NT> __global__ void __launch_bounds__(256) qkv_pool_ke
 
 struct AttnPlan {
   int64_t splits, ztiles, cols;
-  int columns;  // 4 (SPLIT), 8 or 16 query rows a warp
+  int columns;  // 4 (SPLIT) or 8 query rows a warp
   size_t ml_bytes, acc_bytes, scores_bytes, probs_bytes, topk_bytes, total;
 };
 
@@ -1447,12 +1388,12 @@ int check_attn(const bb_qkv_attn_args* a, const char* what, bool need_v) {
 }
 
 // The splits of the key list: one wave of CTAs, one a SM, and no more than one step of 32 keys a warp. Up to 4
-// query rows share products (SPLIT, d = 64 or 128), up to 8 take one column tile, more go 16 at a time.
+// query rows share products (SPLIT, d = 64 or 128), more go 8 at a time.
 void plan_grid(const bb_qkv_attn_args* a, int64_t steps, bool decode, AttnPlan* pl) {
   pl->cols = a->heads / a->cache.kv_heads * a->t;
-  pl->columns = pl->cols <= 4 && a->cache.d % 64 == 0 ? 4 : (pl->cols <= 8 ? 8 : 16);
+  pl->columns = pl->cols <= 4 && a->cache.d % 64 == 0 ? 4 : 8;
   pl->ztiles = cdiv(pl->cols, (int64_t)pl->columns);
-  const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 16 ? warps<4, false, 2>() : (pl->columns == 8 || a->cache.bits == 8 ? warps<8, true, 1>() : warps<4, true, 1>()));
+  const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 8 || a->cache.bits == 8 ? warps<8, true>() : warps<4, true>());
   const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() / (a->cache.kv_heads * pl->ztiles));
   pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(steps, w), (int64_t)1024}));
 }
@@ -1484,7 +1425,7 @@ int plan_route(const bb_qkv_attn_args* a, AttnPlan* pl) {
   *pl = {};
   plan_grid(a, cdiv(a->n_dev ? a->cache.cap : a->n, (int64_t)32), false, pl);
   pl->ml_bytes = align_up((size_t)(a->heads * pl->splits) * 8, 256);
-  // a step of 32 keys: 4 (SPLIT), 8 or 16 scores a key and ztile
+  // a step of 32 keys: 4 (SPLIT) or 8 scores a key and ztile
   pl->scores_bytes = (size_t)(a->cache.kv_heads * cdiv(a->cache.cap, (int64_t)32) * pl->ztiles * pl->columns) * 128;
   pl->probs_bytes = a->out_probs ? 0 : align_up((size_t)(a->cache.kv_heads * a->cache.cap) * 4, 256);
   pl->topk_bytes = align_up(topk_scratch_bytes(a->cache.kv_heads, a->cache.cap, a->route_k), 256);
@@ -1521,17 +1462,17 @@ AttnParams make_params(const bb_qkv_attn_args* a, const AttnPlan& pl, char* ws) 
   return p;
 }
 
-template <bool DECODE, int BITS, int G, int NG, bool SPLIT, int NT>
+template <bool DECODE, int BITS, int G, int NG, bool SPLIT>
 int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
   const dim3 grid((unsigned)(p.splits * p.ztiles), (unsigned)kv_heads);
   if constexpr (DECODE) {
-    const size_t smem = partial_smem<BITS, G, NG, SPLIT, NT>(p.splits);
-    auto* kernel = qkv_partial_kernel<BITS, G, NG, SPLIT, NT>;
+    const size_t smem = partial_smem<BITS, G, NG, SPLIT>(p.splits);
+    auto* kernel = qkv_partial_kernel<BITS, G, NG, SPLIT>;
     if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    kernel<<<grid, 32 * warps<BITS, SPLIT, NT>(), smem, stream>>>(p);
+    kernel<<<grid, 32 * warps<BITS, SPLIT>(), smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_partial_kernel");
     if (p.splits > 1 && !p.tickets) {
-      constexpr int COLS = Layout<SPLIT, NT>::COLS;
+      constexpr int COLS = Layout<SPLIT>::COLS;
       const size_t merge = combine_floats<COLS, 256>(p.splits) * 4;
       auto* after = qkv_combine_kernel<COLS, G * 32>;
       if (merge > 48 * 1024) cudaFuncSetAttribute(after, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)merge);
@@ -1540,7 +1481,7 @@ int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
     }
   } else {
     constexpr size_t smem = (size_t)SCORE_WARPS * SCORE_STAGES * Stage<BITS, G, NG, false>::BYTES;
-    auto* kernel = qkv_scores_kernel<BITS, G, NG, SPLIT, NT>;
+    auto* kernel = qkv_scores_kernel<BITS, G, NG, SPLIT>;
     if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     kernel<<<grid, 32 * SCORE_WARPS, smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_scores_kernel");
@@ -1548,18 +1489,18 @@ int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
   return BB_OK;
 }
 
-template <bool SPLIT, int NT> int launch_pool(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
+template <bool SPLIT> int launch_pool(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
   cudaLaunchAttribute overlap{};
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)cdiv(p.steps, (int64_t)8 * POOL_STEPS), (unsigned)kv_heads);
   cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = (size_t)p.ztiles * Layout<SPLIT, NT>::COLS * 8;
+  cfg.dynamicSmemBytes = (size_t)p.ztiles * Layout<SPLIT>::COLS * 8;
   cfg.stream = stream;
   cfg.attrs = &overlap;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, qkv_pool_kernel<SPLIT, NT>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, qkv_pool_kernel<SPLIT>, p);
   if (e != cudaSuccess) return fail(BB_ERR_LAUNCH, "qkv_pool_kernel: %s", cudaGetErrorString(e));
   BB_CHECK_LAUNCH("qkv_pool_kernel");
   return BB_OK;
@@ -1568,9 +1509,8 @@ template <bool SPLIT, int NT> int launch_pool(const AttnParams& p, int64_t kv_he
 template <bool DECODE, int BITS, int G, int NG>
 int launch_columns(const AttnParams& p, int columns, int64_t kv_heads, cudaStream_t stream) {
   if constexpr (G % 2 == 0)
-    if (columns == 4) return launch<DECODE, BITS, G, NG, true, 1>(p, kv_heads, stream);
-  return columns == 8 ? launch<DECODE, BITS, G, NG, false, 1>(p, kv_heads, stream)
-                      : launch<DECODE, BITS, G, NG, false, 2>(p, kv_heads, stream);
+    if (columns == 4) return launch<DECODE, BITS, G, NG, true>(p, kv_heads, stream);
+  return launch<DECODE, BITS, G, NG, false>(p, kv_heads, stream);
 }
 
 template <bool DECODE, int BITS>
@@ -1636,9 +1576,8 @@ int qkv_route(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_t
   AttnParams p = make_params(a, pl, w);
   st = launch_attn<false>(a, p, pl.columns, stream);
   if (st) return st;
-  st = pl.columns == 4 ? launch_pool<true, 1>(p, a->cache.kv_heads, stream)
-                       : (pl.columns == 8 ? launch_pool<false, 1>(p, a->cache.kv_heads, stream)
-                                          : launch_pool<false, 2>(p, a->cache.kv_heads, stream));
+  st = pl.columns == 4 ? launch_pool<true>(p, a->cache.kv_heads, stream)
+                       : launch_pool<false>(p, a->cache.kv_heads, stream);
   if (st) return st;
   if (a->route_k > 0 && a->out_idx)
     return topk_sorted(p.probs, a->cache.kv_heads, a->cache.cap, a->route_k, a->out_idx, a->out_idx_i64 != 0, a->so_i,

@@ -250,7 +250,7 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
         a.idx_i64 = int(indices.dtype == torch.int64)
     L, size, ref = _lib.lib(), C.c_size_t(0), C.byref(a)
     _lib.check(L.bb_qkv_decode_workspace_size(ref, C.byref(size)), "quant_decode")
-    need = kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 16)
+    need = kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 8)
     tickets, ws = kv._take_scratch(stream, need, size.value)
     a.tickets, a.n_tickets = tickets.data_ptr(), need
     _lib.check(L.bb_qkv_decode(ref, ws.data_ptr(), size.value, stream), "quant_decode")
