@@ -24,6 +24,7 @@
 // maximum of the scores) to at most 2^15, so that p down to 2^-29 of the largest keeps all 11 bits.
 // Scores, exponentials, sums and accumulators are fp32.
 #include <algorithm>
+#include <atomic>
 
 #include "qkv.cuh"
 
@@ -1462,27 +1463,41 @@ AttnParams make_params(const bb_qkv_attn_args* a, const AttnPlan& pl, char* ws) 
   return p;
 }
 
+// Lets a kernel use all of a SM's shared memory: once a device and kernel (the attribute call costs as much host time as
+// a third of a launch).
+template <typename K> int allow_smem(K* kernel, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) dev = -1;
+  if (dev >= 0 && (done.load(std::memory_order_acquire) >> dev & 1)) return BB_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+  if (e != cudaSuccess) return fail(BB_ERR_LAUNCH, "qkv attention: %s", cudaGetErrorString(e));
+  if (dev >= 0) done.fetch_or(uint64_t{1} << dev, std::memory_order_release);
+  return BB_OK;
+}
+
 template <bool DECODE, int BITS, int G, int NG, bool SPLIT>
 int launch(const AttnParams& p, int64_t kv_heads, cudaStream_t stream) {
   const dim3 grid((unsigned)(p.splits * p.ztiles), (unsigned)kv_heads);
   if constexpr (DECODE) {
     const size_t smem = partial_smem<BITS, G, NG, SPLIT>(p.splits);
     auto* kernel = qkv_partial_kernel<BITS, G, NG, SPLIT>;
-    if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> done{0};
+    const int st = allow_smem(kernel, done);
+    if (st) return st;
     kernel<<<grid, 32 * warps<BITS, SPLIT>(), smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_partial_kernel");
     if (p.splits > 1 && !p.tickets) {
       constexpr int COLS = Layout<SPLIT>::COLS;
-      const size_t merge = combine_floats<COLS, 256>(p.splits) * 4;
-      auto* after = qkv_combine_kernel<COLS, G * 32>;
-      if (merge > 48 * 1024) cudaFuncSetAttribute(after, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)merge);
-      after<<<dim3((unsigned)p.ztiles, (unsigned)kv_heads), 256, merge, stream>>>(p);
+      const size_t merge = combine_floats<COLS, 256>(p.splits) * 4;  // at most 36 KB (1024 splits)
+      qkv_combine_kernel<COLS, G * 32><<<dim3((unsigned)p.ztiles, (unsigned)kv_heads), 256, merge, stream>>>(p);
       BB_CHECK_LAUNCH("qkv_combine_kernel");
     }
   } else {
     constexpr size_t smem = (size_t)SCORE_WARPS * SCORE_STAGES * Stage<BITS, G, NG, false>::BYTES;
     auto* kernel = qkv_scores_kernel<BITS, G, NG, SPLIT>;
-    if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> done{0};
+    const int st = allow_smem(kernel, done);
+    if (st) return st;
     kernel<<<grid, 32 * SCORE_WARPS, smem, stream>>>(p);
     BB_CHECK_LAUNCH("qkv_scores_kernel");
   }

@@ -103,13 +103,14 @@ class QuantKV:
         self._scratch = {}
 
     def _take_scratch(self, stream, tickets, nbytes):
+        """Tickets and a workspace of at least these sizes, for a call on ``stream``."""
         if torch.cuda.is_current_stream_capturing():
             return (torch.zeros(tickets, dtype=torch.int32, device=self.device),
                     torch.empty(nbytes, dtype=torch.uint8, device=self.device))
         s = self._scratch.get(stream)
         if s is None or s[0].numel() < tickets or s[1].numel() < nbytes:
             s = self._scratch[stream] = (torch.zeros(max(tickets, 1024), dtype=torch.int32, device=self.device),
-                                         torch.empty(nbytes, dtype=torch.uint8, device=self.device))
+                                         torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device))
         return s
 
     @property
@@ -143,12 +144,11 @@ class QuantKV:
                 raise ValueError(f"QuantKV.write: rows [{at}, {at + t}) outside a cache of {self.capacity}")
         out = None
         if values:
-            both = torch.empty((2, t, hk, d), dtype=k.dtype, device=self.device)
-            a.out_k = first = both.data_ptr()
-            a.out_v = first + t * hk * d * k.element_size()
+            shape, stride = (hk, t, d), (d, hk * d, 1)
+            out = k.new_empty_strided(shape, stride), k.new_empty_strided(shape, stride)
+            a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
             a.sok_h = a.sov_h = d
             a.sok_t = a.sov_t = hk * d
-            out = both.transpose(1, 2).unbind(0)
         _lib.check(_lib.lib().bb_qkv_write(C.byref(a), _stream(self.device)), "QuantKV.write")
         return out
 
@@ -175,15 +175,15 @@ class QuantKV:
             a.positions = positions.data_ptr() if rows else None
             a.sp_h, a.pos_i64 = positions.stride(0), int(positions.dtype == torch.int64)
         hk, d = self.kv_heads, self.head_dim
-        both = torch.empty((2, hk, rows, d), dtype=dtype, device=self.device)
+        shape, stride = (hk, rows, d), (rows * d, d, 1)
+        out = tuple(torch.empty_strided(shape, stride, dtype=dtype, device=self.device) for _ in "kv")
         if rows:
             a.rows = rows
-            a.out_k = first = both.data_ptr()
-            a.out_v = first + hk * rows * d * both.element_size()
+            a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
             a.sok_h = a.sov_h = rows * d
             a.sok_t = a.sov_t = d
             _lib.check(_lib.lib().bb_qkv_read(C.byref(a), _stream(self.device)), "QuantKV.read")
-        return both.unbind(0)
+        return out
 
 
 def _args(q, kv, front, window, scale, n, splits, what):
@@ -231,12 +231,14 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
         if not t or (keep[1] is None and t > a.n):
             raise ValueError("quant_decode: the tokens of q must be among the first n cached")
         a.t, a.sq_t = t, q.stride(1)
-        out = torch.empty((t, h, d), dtype=q.dtype, device=q.device)
+        out = torch.empty_strided((h, t, d), (d, h * d, 1), dtype=q.dtype, device=q.device)
         a.so_h, a.so_t = d, h * d
     else:
-        h, d = q.shape
-        out = torch.empty((h, d), dtype=q.dtype, device=q.device)
-        a.so_h = d
+        h = q.shape[0]
+        out = torch.empty_like(q)
+        if out.stride(-1) != 1:
+            out = out.contiguous()
+        a.so_h = out.stride(0)
     a.out = out.data_ptr()
     stream = _stream(kv.device)
     if indices is not None and indices.shape[-1]:
@@ -248,13 +250,19 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
             indices = indices.contiguous()
         a.idx, a.si_r, a.route_rows, a.route_k = indices.data_ptr(), indices.stride(0), *indices.shape
         a.idx_i64 = int(indices.dtype == torch.int64)
-    L, size, ref = _lib.lib(), C.c_size_t(0), C.byref(a)
-    _lib.check(L.bb_qkv_decode_workspace_size(ref, C.byref(size)), "quant_decode")
+    L, ref = _lib.lib(), C.byref(a)
     need = kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 8)
-    tickets, ws = kv._take_scratch(stream, need, size.value)
+    tickets, ws = kv._take_scratch(stream, need, 1)
     a.tickets, a.n_tickets = tickets.data_ptr(), need
-    _lib.check(L.bb_qkv_decode(ref, ws.data_ptr(), size.value, stream), "quant_decode")
-    return out if q.ndim == 2 else out.transpose(0, 1)
+    status = L.bb_qkv_decode(ref, ws.data_ptr(), ws.numel(), stream)
+    if status == _lib.BB_ERR_WORKSPACE:
+        size = C.c_size_t(0)
+        _lib.check(L.bb_qkv_decode_workspace_size(ref, C.byref(size)), "quant_decode")
+        tickets, ws = kv._take_scratch(stream, need, size.value)
+        a.tickets = tickets.data_ptr()
+        status = L.bb_qkv_decode(ref, ws.data_ptr(), ws.numel(), stream)
+    _lib.check(status, "quant_decode")
+    return out
 
 
 def _route(a, kv, what):
