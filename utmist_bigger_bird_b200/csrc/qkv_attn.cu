@@ -724,14 +724,13 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
     const int r = lane / 4, c = lane % 4;
     float s[2][4], e[2][4], f[2], shrink;
     step_scores<BITS, G, NG, SPLIT>(q, st, st + S::KM, lane, s);
-    uint32_t m0[2][NG], m1[2][NG];
     float smax = 0.f;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      lds_words(m0[x], st + S::VM + (x * 16 + r) * S::META);
-      lds_words(m1[x], st + S::VM + (x * 16 + r + 8) * S::META);
+    for (int i = 0; i < 4; ++i) {
+      uint32_t m[NG];
+      lds_words(m, st + S::VM + (i * 8 + r) * S::META);
 #pragma unroll
-      for (int gi = 0; gi < NG; ++gi) smax = fmax3(smax, step_of(m0[x][gi]), step_of(m1[x][gi]));  // NaN ignored
+      for (int gi = 0; gi < NG; ++gi) smax = fmaxf(smax, step_of(m[gi]));  // NaN ignored
     }
     if (run.template update<EDGE>(e, s, q.mul, mask, smax, f, shrink)) {
 #pragma unroll
@@ -743,13 +742,15 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
 #pragma unroll
       for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[i / 4][i % 4] *= f[i & 1] * shrink;
     }
-    uint32_t b[NG][2][2];
 #pragma unroll
-    for (int gi = 0; gi < NG; ++gi)
+    for (int x = 0; x < 2; ++x) {
+      uint32_t m0[NG], m1[NG], b[NG][2];
+      lds_words(m0, st + S::VM + (x * 16 + r) * S::META);
+      lds_words(m1, st + S::VM + (x * 16 + r + 8) * S::META);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float s0 = step_of(m0[x][gi]), s1 = step_of(m1[x][gi]);
-        const float h0 = fmaf(CENTRE<BITS>, s0, low_of(m0[x][gi])), h1 = fmaf(CENTRE<BITS>, s1, low_of(m1[x][gi]));
+      for (int gi = 0; gi < NG; ++gi) {
+        const float s0 = step_of(m0[gi]), s1 = step_of(m1[gi]);
+        const float h0 = fmaf(CENTRE<BITS>, s0, low_of(m0[gi])), h1 = fmaf(CENTRE<BITS>, s1, low_of(m1[gi]));
         const float t0 = s0 * run.pscale, t1 = s1 * run.pscale;
         float u[4] = {e[x][0] * t0, e[x][1] * t0, e[x][2] * t1, e[x][3] * t1};
         if constexpr (EDGE) {  // rows that do not count may hold NaN
@@ -765,13 +766,11 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
           mid[gi][0] = fmaf(e[x][0], h0, fmaf(e[x][2], h1, mid[gi][0]));
           mid[gi][1] = fmaf(e[x][1], h0, fmaf(e[x][3], h1, mid[gi][1]));
         }
-        b[gi][x][0] = transpose8(pack2<__half>(u[0], u[1]));
-        b[gi][x][1] = transpose8(pack2<__half>(u[2], u[3]));
-        mma_sum(ps[gi / 2], gi % 2, b[gi][x][0]);
-        mma_sum(ps[gi / 2], gi % 2, b[gi][x][1]);
+        b[gi][0] = transpose8(pack2<__half>(u[0], u[1]));
+        b[gi][1] = transpose8(pack2<__half>(u[2], u[3]));
+        mma_sum(ps[gi / 2], gi % 2, b[gi][0]);
+        mma_sum(ps[gi / 2], gi % 2, b[gi][1]);
       }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
       uint32_t w[4][VW];  // rows c, c + 4 (slots 2c, 2c + 1) and c + 8, c + 12 (slots 2c + 8, 2c + 9)
 #pragma unroll
       for (int i = 0; i < 4; ++i) v_words<BITS, G>(w[i], st + S::V, x * 16 + c + 4 * i, r);
@@ -779,8 +778,8 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
       for (int g = 0; g < G; ++g) {
         uint32_t a[2][4];
         operands(a, w, g);
-        mma_h(o[g][0], a[0], b[g / (G / NG)][x]);
-        mma_h(o[g][1], a[1], b[g / (G / NG)][x]);
+        mma_h(o[g][0], a[0], b[g / (G / NG)]);
+        mma_h(o[g][1], a[1], b[g / (G / NG)]);
       }
     }
   }
