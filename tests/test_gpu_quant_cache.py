@@ -294,6 +294,29 @@ def test_pooled_probs(bits, d, group, g, dtype, n, front, window):
         assert (np.abs(got - want)[live] <= want[live] * (2.0 ** -18 * reach + 2.0 ** -17) + 1e-37).all()
 
 
+@pytest.mark.parametrize("g", [4, 8, 12])
+@pytest.mark.parametrize("splits", [1, 3, 1000])
+def test_pooled_probs_explicit_splits(splits, g):
+    """Few splits: more scores a warp than its CTA keeps. The same bits with and without the one-launch path (calls under
+    a graph capture take two launches); more query heads than one column tile."""
+    from utmist_bigger_bird_b200 import quant_pooled_probs
+    hk, cap, d, n = 2, 20000, 128, 19990
+    kv, kval, _, _ = filled(hk, cap, d)
+    q = rand((hk * g, 1, d), 29)[:, 0]
+    kw = dict(front=5, window=77, scale=d ** -0.5, n=n, splits=splits)
+    got = quant_pooled_probs(q, kv, **kw)
+    want = qo.pooled_probs(f64(q), kval, front=5, window=77, scale=d ** -0.5, n=n, cap=cap)
+    reach = np.abs(f64(q)).sum(-1).max() * np.abs(kval).max() * d ** -0.5
+    live = want != -1
+    assert ((f64(got) == -1) == ~live).all()
+    assert (np.abs(f64(got) - want)[live] <= want[live] * (2.0 ** -18 * reach + 2.0 ** -17) + 1e-37).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = quant_pooled_probs(q, kv, **kw)
+    graph.replay()
+    assert torch.equal(again, got)
+
+
 def test_route_picks_its_own_top_probabilities():
     from utmist_bigger_bird_b200 import quant_pooled_probs, quant_route
     kv, *_ = filled(cap=5000)

@@ -72,6 +72,8 @@ int qkv_decode_workspace_size(const bb_qkv_attn_args* a, size_t* bytes);
 int qkv_decode(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_t stream);
 int qkv_route_workspace_size(const bb_qkv_attn_args* a, size_t* bytes);
 int qkv_route(const bb_qkv_attn_args* a, void* ws, size_t ws_bytes, cudaStream_t stream);
+int qkv_fault_take(int* code);
+int qkv_set_wait_limit(unsigned long long ns);
 
 namespace {
 
@@ -176,20 +178,23 @@ uint64_t bb_kernel_launches(void) { return bb::g_launches.load(std::memory_order
 
 int bb_device_fault(int* code) {
   if (!code) return bb::fail(BB_ERR_ARG, "device_fault: null pointer");
-  int a = 0, b = 0, c = 0;
+  int a = 0, b = 0, c = 0, d = 0;
   int st = bb::flash_fault_take(&a);
   if (st != BB_OK) return st;
   st = bb::routes_fault_take(&b);
   if (st != BB_OK) return st;
   st = bb::decode_fault_take(&c);
   if (st != BB_OK) return st;
-  *code = a ? a : (b ? b : c);
+  st = bb::qkv_fault_take(&d);
+  if (st != BB_OK) return st;
+  *code = a ? a : (b ? b : (c ? c : d));
   return BB_OK;
 }
 
 int bb_set_wait_limit_ns(uint64_t ns) {
   if (ns == 0) return bb::fail(BB_ERR_ARG, "set_wait_limit_ns: the limit must be positive");
-  if (bb::flash_set_wait_limit(ns) || bb::routes_set_wait_limit(ns) || bb::decode_set_wait_limit(ns))
+  if (bb::flash_set_wait_limit(ns) || bb::routes_set_wait_limit(ns) || bb::decode_set_wait_limit(ns) ||
+      bb::qkv_set_wait_limit(ns))
     return bb::fail(BB_ERR_LAUNCH, "set_wait_limit_ns: %s", cudaGetErrorString(cudaGetLastError()));
   return BB_OK;
 }

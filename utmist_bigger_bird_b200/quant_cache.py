@@ -266,10 +266,12 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
 
 
 def _route(a, kv, what):
-    L, size, ref = _lib.lib(), C.c_size_t(0), C.byref(a)
+    L, size, ref, stream = _lib.lib(), C.c_size_t(0), C.byref(a), _stream(kv.device)
     _lib.check(L.bb_qkv_route_workspace_size(ref, C.byref(size)), what)
     ws = torch.empty(size.value, dtype=torch.uint8, device=kv.device)
-    _lib.check(L.bb_qkv_route(ref, ws.data_ptr(), size.value, _stream(kv.device)), what)
+    if not torch.cuda.is_current_stream_capturing():
+        a.tickets, a.n_tickets = kv._take_scratch(stream, 2 * kv.kv_heads, 1)[0].data_ptr(), 2 * kv.kv_heads
+    _lib.check(L.bb_qkv_route(ref, ws.data_ptr(), size.value, stream), what)
 
 
 def quant_pooled_probs(q, kv, *, front=64, window=4096, scale=1.0, n=None, splits=None):
