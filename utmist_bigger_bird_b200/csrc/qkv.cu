@@ -6,6 +6,10 @@
 // Both are bound by HBM: a row of d 16-bit values is 2 d bytes on one side and d bits / 8 + 4 d / group
 // on the other. A thread owns 16 consecutive dimensions (32 bytes of a 16-bit row); a group's
 // minimum and maximum come from shuffles among the 2, 4, 6 or 8 threads that share it.
+// Measured, 128K rows of 8 heads, d = 128, 4 bits, groups of 32, bf16: writing with the values returned (1.24 GB) 221 us,
+// reading (705 MB) 112 us, 86 % and 97 % of a copy's rate. On the way: 8 dimensions and 4 rows a thread 299 and 131 us
+// (group and address work is shared by fewer dimensions); 16 dimensions in 16-byte accesses 232 and 145 us (each access
+// touches half a sector); scalar fp32 arithmetic with library division 369 and 196 us.
 #include <algorithm>
 
 #include "qkv.cuh"
