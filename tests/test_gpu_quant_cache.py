@@ -363,6 +363,27 @@ def test_results_do_not_depend_on_stream_or_repetition():
     assert torch.equal(kv.read(start=2500, stop=2501)[0], kv.read(start=2502, stop=2503)[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_unaligned_rows(dtype):
+    """Queries and new rows that start at odd addresses or have odd strides."""
+    from utmist_bigger_bird_b200 import QuantKV
+    c = filled(dtype=dtype)
+    flat = rand((1, 1, 8 * 131 + 1), 30, dtype).flatten()
+    q = flat[1:].as_strided((8, 128), (131, 1), 1)
+    check_decode(*c, q, None, 290, 4, 40, dtype)
+    q = rand((8, 128, 3), 31, dtype).transpose(1, 2)      # dimensions three elements apart
+    check_decode(*c, q, None, 290, 4, 40, dtype)
+    x = rand((2, 5, 131), 32, dtype)[..., 1:129]
+    a, b = QuantKV(2, 5, 128), QuantKV(2, 5, 128)
+    a.write(x, x, 0)
+    b.write(x.contiguous(), x.contiguous(), 0)
+    assert torch.equal(a.k_codes, b.k_codes) and torch.equal(a.v_meta, b.v_meta)
+    # rows on 16-byte but not on 32-byte boundaries
+    y = torch.empty(2 * 5 * 136 + 8, dtype=dtype, device=DEV)[8:].view(2, 5, 136)[..., :128].copy_(x)
+    vals = b.write(y, y, 0, values=True)
+    assert torch.equal(a.k_codes, b.k_codes) and torch.equal(vals[0], a.read(dtype=dtype)[0])
+
+
 def test_buffers_with_gaps_between_heads():
     """Heads that lie further apart than their rows (a view of a longer cache)."""
     from utmist_bigger_bird_b200 import QuantKV

@@ -73,6 +73,7 @@ def attn(cache_kw=None, **kw):
     (dict(group=16), {}, 2, "group"),
     (dict(kv_heads=0), {}, 2, "kv_heads"),
     (dict(cap=0), {}, 2, "capacity"),
+    (dict(cap=2 ** 31 - 64), {}, 2, "capacity"),
     (dict(k_meta=None), {}, 1, "null"),
     (dict(v_codes=BUF + 8), {}, 4, "16-byte"),
     (dict(k_codes_h=64 * 99), {}, 4, "overlap"),
@@ -155,6 +156,8 @@ def test_wrapper_refusals():
     for kw in (dict(start=-1), dict(start=4, stop=3), dict(stop=11), dict(dtype=torch.float64)):
         with pytest.raises(ValueError):
             kv.read(**kw)
+    with pytest.raises(ValueError, match="CUDA"):
+        kv.read()
     for pos in (torch.zeros(3, 4, dtype=torch.int64), torch.zeros(2, 4), torch.zeros(2, dtype=torch.int32)):
         with pytest.raises(ValueError):
             kv.read(pos)

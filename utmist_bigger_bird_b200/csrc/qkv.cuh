@@ -19,7 +19,8 @@ inline int check_cache(const bb_qkv_cache& c, const char* what, bool need_k, boo
   if (c.group <= 0 || c.group % 32 || c.d % c.group)
     return fail(BB_ERR_SHAPE, "%s: group must be a multiple of 32 that divides head_dim", what);
   if (c.kv_heads <= 0 || c.kv_heads > 65535) return fail(BB_ERR_SHAPE, "%s: kv_heads must lie in [1, 65535]", what);
-  if (c.cap <= 0 || c.cap > INT32_MAX) return fail(BB_ERR_SHAPE, "%s: capacity must lie in [1, 2^31)", what);
+  if (c.cap <= 0 || c.cap > INT32_MAX - 64)  // positions rounded up to a step of 32 stay below 2^31
+    return fail(BB_ERR_SHAPE, "%s: capacity must lie in [1, 2^31 - 65]", what);
   const int64_t row = c.d * c.bits / 8, pairs = c.d / c.group;
   if ((need_k && (!c.k_codes || !c.k_meta)) || (need_v && (!c.v_codes || !c.v_meta)))
     return fail(BB_ERR_ARG, "%s: null cache buffer", what);

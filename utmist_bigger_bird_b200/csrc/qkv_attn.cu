@@ -1182,16 +1182,16 @@ __global__ void __launch_bounds__(32 * warps<BITS, SPLIT>(), 1) qkv_partial_kern
   }
   if (p.splits == 1 || !p.tickets) return;
   // The last CTA of the tile to arrive merges its splits, always in the same order.
-  __threadfence();
-  __syncthreads();
   __shared__ bool last;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    __threadfence();  // the barrier's writes before it, of all threads, and the counter's after
     last = atomicAdd(p.tickets + tile, 1) == p.splits - 1;
     if (last) p.tickets[tile] = 0;
+    __threadfence();
   }
   __syncthreads();
   if (!last) return;
-  __threadfence();
   combine<Y::COLS, D, 32 * W>(p, tile, kv, col0, reinterpret_cast<float*>(smem));
 }
 
@@ -1375,12 +1375,13 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 1) qkv_scores_kernel(const A
     __shared__ float2 stats[Y::COLS];
     __shared__ bool all;
     int32_t* arrived = p.tickets + 2 * kv;  // and [1]: those that have seen all arrive
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+      __threadfence();  // the barrier's writes before it, of all threads
       atomicAdd(arrived, 1);
       all = wait_arrivals(arrived, p.splits);
       if (all && atomicAdd(arrived + 1, 1) == p.splits - 1) arrived[0] = arrived[1] = 0;
+      __threadfence();
     }
     __syncthreads();
     if (!all) return;

@@ -157,6 +157,8 @@ class QuantKV:
         cache give zeros): (k, v) [Hkv, L, d]."""
         if dtype not in _ops._DT:
             raise ValueError("QuantKV.read: dtype must be one of f16/bf16/f32")
+        if self.device.type != "cuda":
+            raise ValueError("QuantKV.read requires a CUDA cache")
         a = _lib.QkvReadArgs.from_buffer_copy(self._read)
         a.dtype = _ops._DT[dtype]
         if positions is None:
