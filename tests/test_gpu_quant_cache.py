@@ -141,6 +141,12 @@ def test_write_at_device_position_and_edges():
 
 @pytest.mark.parametrize("dt", [torch.int32, torch.int64])
 def test_read_positions(dt):
+    small, *_ = filled()
+    for kw in (dict(start=-1), dict(start=4, stop=3), dict(stop=301), dict(dtype=torch.float64),
+               dict(positions=torch.zeros(3, 4, dtype=dt, device=DEV)), dict(positions=torch.zeros(2, 4, device=DEV)),
+               dict(positions=torch.zeros(2, dtype=dt, device=DEV)), dict(positions=torch.zeros(2, 4, dtype=dt))):
+        with pytest.raises(ValueError):
+            small.read(**kw)
     kv, kval, vval, _ = filled(hk=3, cap=200, d=96, bits=8, group=96)
     pos = torch.randint(0, 200, (3, 77), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dt)
     pos[0, 0], pos[1, 5] = -1, 200                        # outside: zeros
@@ -297,9 +303,12 @@ def test_pooled_probs(bits, d, group, g, dtype, n, front, window):
 @pytest.mark.parametrize("g", [4, 8, 12])
 @pytest.mark.parametrize("splits", [1, 3, 1000])
 def test_pooled_probs_explicit_splits(splits, g):
-    """Few splits: more scores a warp than its CTA keeps. The same bits with and without the one-launch path (calls under
-    a graph capture take two launches); more query heads than one column tile."""
-    from utmist_bigger_bird_b200 import quant_pooled_probs
+    """Few splits: more scores a warp than its CTA keeps. The same bits in one launch, under a graph capture, and in two
+    launches (a call without tickets); more query heads than one column tile."""
+    import ctypes as C
+
+    from utmist_bigger_bird_b200 import _lib, quant_pooled_probs
+    from utmist_bigger_bird_b200.quant_cache import _args
     hk, cap, d, n = 2, 20000, 128, 19990
     kv, kval, _, _ = filled(hk, cap, d)
     q = rand((hk * g, 1, d), 29)[:, 0]
@@ -315,6 +324,38 @@ def test_pooled_probs_explicit_splits(splits, g):
         again = quant_pooled_probs(q, kv, **kw)
     graph.replay()
     assert torch.equal(again, got)
+    a, _ = _args(q, kv, kw["front"], kw["window"], kw["scale"], n, splits, "probs")
+    two, size = torch.zeros_like(got), C.c_size_t(0)
+    a.out_probs = two.data_ptr()
+    _lib.check(_lib.lib().bb_qkv_route_workspace_size(C.byref(a), C.byref(size)), "probs")
+    ws = torch.empty(size.value, dtype=torch.uint8, device=DEV)
+    _lib.check(_lib.lib().bb_qkv_route(C.byref(a), ws.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream), "probs")
+    assert torch.equal(two, got)
+
+
+def test_decode_without_tickets_takes_two_launches():
+    """The C entry without tickets merges in a second launch, with the same result."""
+    import ctypes as C
+
+    from utmist_bigger_bird_b200 import _lib, quant_decode
+    from utmist_bigger_bird_b200.quant_cache import _args
+    L = _lib.lib()
+    for g, bits, d, group in ((4, 4, 128, 32), (7, 8, 96, 96)):
+        kv, *_ = filled(2, 3000, d, bits, group)
+        q = rand((2 * g, 1, d), 33)[:, 0]
+        kw = dict(front=3, window=2000, scale=0.1, n=2990)
+        before = L.bb_kernel_launches()
+        want = quant_decode(q, kv, **kw)
+        one = L.bb_kernel_launches() - before
+        a, _ = _args(q, kv, kw["front"], kw["window"], kw["scale"], kw["n"], None, "decode")
+        out, size = torch.zeros_like(want), C.c_size_t(0)
+        a.out, a.so_h = out.data_ptr(), d
+        _lib.check(L.bb_qkv_decode_workspace_size(C.byref(a), C.byref(size)), "decode")
+        ws = torch.empty(size.value, dtype=torch.uint8, device=DEV)
+        before = L.bb_kernel_launches()
+        _lib.check(L.bb_qkv_decode(C.byref(a), ws.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream), "decode")
+        assert (one, L.bb_kernel_launches() - before) == (1, 2)
+        assert torch.equal(out, want)
 
 
 def test_route_picks_its_own_top_probabilities():

@@ -22,7 +22,7 @@ from . import _lib, _ops
 
 __all__ = ["QuantKV", "quant_decode", "quant_pooled_probs", "quant_route"]
 
-_HALF = (torch.float16, torch.bfloat16)
+_HALF = {torch.float16: _lib.BB_F16, torch.bfloat16: _lib.BB_BF16}
 
 
 def _rows(x):
@@ -39,6 +39,40 @@ def _rows(x):
 def _stream(device):
     """The current stream's handle (``torch.cuda.current_stream`` builds a Stream object for it)."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+# Counters (zero between calls) and a workspace, a pair a stream, for calls that run one after the other on it. They grow to
+# the largest call's and stay.
+_scratch = {}
+
+
+def _take_scratch(device, stream, tickets, nbytes):
+    """Tickets and a workspace of at least these sizes for a call on ``stream``. Calls under a graph capture get their own,
+    which the graph zeroes and keeps."""
+    if torch.cuda.is_current_stream_capturing():
+        return (torch.zeros(tickets, dtype=torch.int32, device=device),
+                torch.empty(nbytes, dtype=torch.uint8, device=device))
+    s = _scratch.get((device.index, stream))
+    if s is None or s[0].numel() < tickets or s[1].numel() < nbytes:
+        s = _scratch[device.index, stream] = (torch.zeros(max(tickets, 1024), dtype=torch.int32, device=device),
+                                              torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device))
+    return s
+
+
+def _run(what, run, size_of, a, device, stream, tickets):
+    """One call of a C entry that takes a workspace: with the stream's, or a larger one if that is too small."""
+    ref = C.byref(a)
+    t, ws = _take_scratch(device, stream, tickets, 1)
+    a.tickets, a.n_tickets = t.data_ptr(), tickets
+    status = run(ref, ws.data_ptr(), ws.numel(), stream)
+    if status == _lib.BB_ERR_WORKSPACE:
+        size = C.c_size_t(0)
+        _lib.check(size_of(ref, C.byref(size)), what)
+        t, ws = _take_scratch(device, stream, tickets, size.value)
+        a.tickets = t.data_ptr()
+        status = run(ref, ws.data_ptr(), ws.numel(), stream)
+    if status:
+        _lib.check(status, what)
 
 
 class QuantKV:
@@ -98,20 +132,6 @@ class QuantKV:
         self._attn = _lib.QkvAttnArgs(cache=self._struct)
         self._write = _lib.QkvWriteArgs(cache=self._struct)
         self._read = _lib.QkvReadArgs(cache=self._struct)
-        # Counters (zero between calls) and workspace of quant_decode, a pair a stream: calls on one stream do not
-        # overlap. Calls under a graph capture get their own, which the graph keeps.
-        self._scratch = {}
-
-    def _take_scratch(self, stream, tickets, nbytes):
-        """Tickets and a workspace of at least these sizes, for a call on ``stream``."""
-        if torch.cuda.is_current_stream_capturing():
-            return (torch.zeros(tickets, dtype=torch.int32, device=self.device),
-                    torch.empty(nbytes, dtype=torch.uint8, device=self.device))
-        s = self._scratch.get(stream)
-        if s is None or s[0].numel() < tickets or s[1].numel() < nbytes:
-            s = self._scratch[stream] = (torch.zeros(max(tickets, 1024), dtype=torch.int32, device=self.device),
-                                         torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device))
-        return s
 
     @property
     def nbytes(self):
@@ -122,21 +142,23 @@ class QuantKV:
         1-element GPU integer tensor (rows that fall outside the cache are then skipped). With
         ``values``, returns what the rows now stand for, (k, v) [Hkv, T, d] in the input dtype, stored
         as [T, Hkv, d]."""
-        if not k.is_cuda or k.device != self.device or v.device != self.device:
+        dev = self.device
+        if k.device != dev or v.device != dev or dev.type != "cuda":
             raise ValueError("QuantKV.write requires CUDA tensors on the cache's device")
         dtype = _ops._DT.get(k.dtype)
         if dtype is None or v.dtype != k.dtype:
             raise ValueError("QuantKV.write: k and v must share one of f16/bf16/f32")
-        if k.ndim != 3 or k.shape != v.shape or k.shape[0] != self.kv_heads or k.shape[2] != self.head_dim:
+        shape = k.shape
+        if len(shape) != 3 or v.shape != shape or shape[0] != self.kv_heads or shape[2] != self.head_dim:
             raise ValueError("QuantKV.write: k and v must be [Hkv, T, d] of the cache")
-        hk, t, d = k.shape
+        hk, t, d = shape
         a = _lib.QkvWriteArgs.from_buffer_copy(self._write)
         k, a.k, a.sk_h, a.sk_t = _rows(k)
         v, a.v, a.sv_h, a.sv_t = _rows(v)
         a.t, a.dtype = t, dtype
         keep = None
         if isinstance(at, torch.Tensor):
-            keep = _ops._n_arg(at, 0, self.device)[2]
+            keep = _ops._n_arg(at, 0, dev)[2]
             a.at_dev = keep.data_ptr()
         else:
             a.at = at = int(at)
@@ -144,66 +166,72 @@ class QuantKV:
                 raise ValueError(f"QuantKV.write: rows [{at}, {at + t}) outside a cache of {self.capacity}")
         out = None
         if values:
-            shape, stride = (hk, t, d), (d, hk * d, 1)
+            stride = (d, hk * d, 1)
             out = k.new_empty_strided(shape, stride), k.new_empty_strided(shape, stride)
             a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
             a.sok_h = a.sov_h = d
             a.sok_t = a.sov_t = hk * d
-        _lib.check(_lib.lib().bb_qkv_write(C.byref(a), _stream(self.device)), "QuantKV.write")
+        status = _lib.lib().bb_qkv_write(C.byref(a), _stream(dev))
+        if status:
+            _lib.check(status, "QuantKV.write")
         return out
 
     def read(self, positions=None, *, start=0, stop=None, dtype=torch.bfloat16):
         """Values of rows [start, stop), or of rows ``positions`` (int32 / int64 [Hkv, L]; positions outside the
         cache give zeros): (k, v) [Hkv, L, d]."""
-        if dtype not in _ops._DT:
+        dt, dev = _ops._DT.get(dtype), self.device
+        if dt is None:
             raise ValueError("QuantKV.read: dtype must be one of f16/bf16/f32")
-        if self.device.type != "cuda":
+        if dev.type != "cuda":
             raise ValueError("QuantKV.read requires a CUDA cache")
         a = _lib.QkvReadArgs.from_buffer_copy(self._read)
-        a.dtype = _ops._DT[dtype]
+        hk, d = self.kv_heads, self.head_dim
         if positions is None:
             stop = self.capacity if stop is None else int(stop)
             if not 0 <= start <= stop <= self.capacity:
                 raise ValueError(f"QuantKV.read: rows [{start}, {stop}) outside a cache of {self.capacity}")
             a.start, rows = start, stop - start
         else:
-            if positions.device != self.device or positions.dtype not in (torch.int32, torch.int64):
+            wide = positions.dtype == torch.int64
+            if positions.device != dev or not (wide or positions.dtype == torch.int32):
                 raise ValueError("QuantKV.read: positions must be int32 or int64 on the cache's device")
-            if positions.ndim != 2 or positions.shape[0] != self.kv_heads:
+            if positions.ndim != 2 or positions.shape[0] != hk:
                 raise ValueError("QuantKV.read: positions must be [Hkv, L]")
-            rows = positions.shape[1]
-            if positions.stride(-1) != 1:
+            if positions.stride(1) != 1:
                 positions = positions.contiguous()
-            a.positions = positions.data_ptr() if rows else None
-            a.sp_h, a.pos_i64 = positions.stride(0), int(positions.dtype == torch.int64)
-        hk, d = self.kv_heads, self.head_dim
+            rows = positions.shape[1]
+            a.positions, a.sp_h, a.pos_i64 = positions.data_ptr() if rows else None, positions.stride(0), wide
         shape, stride = (hk, rows, d), (rows * d, d, 1)
-        out = tuple(torch.empty_strided(shape, stride, dtype=dtype, device=self.device) for _ in "kv")
+        k = torch.empty_strided(shape, stride, dtype=dtype, device=dev)
+        v = torch.empty_strided(shape, stride, dtype=dtype, device=dev)
         if rows:
-            a.rows = rows
-            a.out_k, a.out_v = out[0].data_ptr(), out[1].data_ptr()
+            a.dtype, a.rows, a.out_k, a.out_v = dt, rows, k.data_ptr(), v.data_ptr()
             a.sok_h = a.sov_h = rows * d
             a.sok_t = a.sov_t = d
-            _lib.check(_lib.lib().bb_qkv_read(C.byref(a), _stream(self.device)), "QuantKV.read")
-        return out
+            status = _lib.lib().bb_qkv_read(C.byref(a), _stream(dev))
+            if status:
+                _lib.check(status, "QuantKV.read")
+        return k, v
 
 
 def _args(q, kv, front, window, scale, n, splits, what):
     """The filled argument struct of an attention call, and the tensors that must outlive it."""
-    if not q.is_cuda or q.dtype not in _HALF:
+    dtype = _HALF.get(q.dtype)
+    if dtype is None or not q.is_cuda:
         raise ValueError(f"{what} requires CUDA FP16/BF16 queries")
     if q.device != kv.device:
         raise ValueError(f"{what}: q and the cache must be on one device")
-    if q.shape[0] % kv.kv_heads or not q.shape[0] or q.shape[-1] != kv.head_dim:
+    shape, stride = q.shape, q.stride()
+    if not shape[0] or shape[0] % kv.kv_heads or shape[-1] != kv.head_dim:
         raise ValueError(f"{what}: q must be [H, ..., {kv.head_dim}] with H a multiple of {kv.kv_heads}")
     if front < 0 or window < 0:
         raise ValueError(f"{what}: front and window must be >= 0")
-    if q.stride(-1) != 1:
+    if stride[-1] != 1:
         q = q.contiguous()
+        stride = q.stride()
     a = _lib.QkvAttnArgs.from_buffer_copy(kv._attn)
-    a.q, a.sq_h, a.heads = q.data_ptr(), q.stride(0), q.shape[0]
+    a.q, a.sq_h, a.heads, a.dtype = q.data_ptr(), stride[0], shape[0], dtype
     a.t, a.front, a.window, a.scale, a.splits = 1, front, window, scale, splits or 0
-    a.dtype = _ops._DT[q.dtype]
     keep = None
     if isinstance(n, torch.Tensor):
         a.n, a.n_dev, keep = _ops._n_arg(n, kv.capacity, kv.device)
@@ -242,7 +270,6 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
             out = out.contiguous()
         a.so_h = out.stride(0)
     a.out = out.data_ptr()
-    stream = _stream(kv.device)
     if indices is not None and indices.shape[-1]:
         if indices.device != q.device or indices.dtype not in (torch.int32, torch.int64):
             raise ValueError("quant_decode: indices must be int32 or int64 on q's device")
@@ -252,28 +279,15 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
             indices = indices.contiguous()
         a.idx, a.si_r, a.route_rows, a.route_k = indices.data_ptr(), indices.stride(0), *indices.shape
         a.idx_i64 = int(indices.dtype == torch.int64)
-    L, ref = _lib.lib(), C.byref(a)
-    need = kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 8)
-    tickets, ws = kv._take_scratch(stream, need, 1)
-    a.tickets, a.n_tickets = tickets.data_ptr(), need
-    status = L.bb_qkv_decode(ref, ws.data_ptr(), ws.numel(), stream)
-    if status == _lib.BB_ERR_WORKSPACE:
-        size = C.c_size_t(0)
-        _lib.check(L.bb_qkv_decode_workspace_size(ref, C.byref(size)), "quant_decode")
-        tickets, ws = kv._take_scratch(stream, need, size.value)
-        a.tickets = tickets.data_ptr()
-        status = L.bb_qkv_decode(ref, ws.data_ptr(), ws.numel(), stream)
-    _lib.check(status, "quant_decode")
+    L = _lib.lib()
+    _run("quant_decode", L.bb_qkv_decode, L.bb_qkv_decode_workspace_size, a, kv.device, _stream(kv.device),
+         kv.kv_heads * -(-(h // kv.kv_heads * a.t) // 8))
     return out
 
 
 def _route(a, kv, what):
-    L, size, ref, stream = _lib.lib(), C.c_size_t(0), C.byref(a), _stream(kv.device)
-    _lib.check(L.bb_qkv_route_workspace_size(ref, C.byref(size)), what)
-    ws = torch.empty(size.value, dtype=torch.uint8, device=kv.device)
-    if not torch.cuda.is_current_stream_capturing():
-        a.tickets, a.n_tickets = kv._take_scratch(stream, 2 * kv.kv_heads, 1)[0].data_ptr(), 2 * kv.kv_heads
-    _lib.check(L.bb_qkv_route(ref, ws.data_ptr(), size.value, stream), what)
+    L = _lib.lib()
+    _run(what, L.bb_qkv_route, L.bb_qkv_route_workspace_size, a, kv.device, _stream(kv.device), 2 * kv.kv_heads)
 
 
 def quant_pooled_probs(q, kv, *, front=64, window=4096, scale=1.0, n=None, splits=None):
@@ -282,7 +296,8 @@ def quant_pooled_probs(q, kv, *, front=64, window=4096, scale=1.0, n=None, split
     if q.ndim != 2:
         raise ValueError("quant_pooled_probs: q must be [H, d]")
     a, keep = _args(q, kv, front, window, scale, n, splits, "quant_pooled_probs")
-    probs = torch.empty(kv.kv_heads, kv.capacity, dtype=torch.float32, device=kv.device)
+    hk, cap = kv.kv_heads, kv.capacity
+    probs = torch.empty_strided((hk, cap), (cap, 1), dtype=torch.float32, device=kv.device)
     a.out_probs = probs.data_ptr()
     _route(a, kv, "quant_pooled_probs")
     return probs
