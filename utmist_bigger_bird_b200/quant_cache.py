@@ -42,7 +42,8 @@ def _stream(device):
 
 
 # Counters (zero between calls) and a workspace, a pair a stream, for calls that run one after the other on it. They grow to
-# the largest call's and stay.
+# the largest call's and stay. A program that goes on after a fault that bb_device_fault reports clears this first: the
+# counters may have been left above zero.
 _scratch = {}
 
 
