@@ -15,6 +15,7 @@ integer tensors that the kernels read at run time, so a captured CUDA graph foll
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -41,37 +42,41 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-# Counters (zero between calls) and a workspace, a pair a stream, for calls that run one after the other on it. They grow to
-# the largest call's and stay. A program that goes on after a fault that bb_device_fault reports clears this first: the
-# counters may have been left above zero.
+# Counters (zero between calls), a workspace and a lock, one set a stream, for calls that run one after the other on it. They
+# grow to the largest call's and stay. A call holds the lock while it enqueues: its launches hand each other results in the
+# workspace, and a call of another thread on the stream must come after the last of them. A program that goes on after a fault
+# that bb_device_fault reports clears this first: the counters may have been left above zero.
 _scratch = {}
 
 
 def _take_scratch(device, stream, tickets, nbytes):
-    """Tickets and a workspace of at least these sizes for a call on ``stream``. Calls under a graph capture get their own,
-    which the graph zeroes and keeps."""
+    """Tickets and a workspace of at least these sizes for a call on ``stream``, and the lock under which to use them. Calls
+    under a graph capture get their own, which the graph zeroes and keeps."""
     if torch.cuda.is_current_stream_capturing():
         return (torch.zeros(tickets, dtype=torch.int32, device=device),
-                torch.empty(nbytes, dtype=torch.uint8, device=device))
+                torch.empty(nbytes, dtype=torch.uint8, device=device), threading.Lock())
     s = _scratch.get((device.index, stream))
     if s is None or s[0].numel() < tickets or s[1].numel() < nbytes:
         s = _scratch[device.index, stream] = (torch.zeros(max(tickets, 1024), dtype=torch.int32, device=device),
-                                              torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device))
+                                              torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device),
+                                              threading.Lock())
     return s
 
 
 def _run(what, run, size_of, a, device, stream, tickets):
     """One call of a C entry that takes a workspace: with the stream's, or a larger one if that is too small."""
     ref = C.byref(a)
-    t, ws = _take_scratch(device, stream, tickets, 1)
+    t, ws, lock = _take_scratch(device, stream, tickets, 1)
     a.tickets, a.n_tickets = t.data_ptr(), tickets
-    status = run(ref, ws.data_ptr(), ws.numel(), stream)
+    with lock:
+        status = run(ref, ws.data_ptr(), ws.numel(), stream)
     if status == _lib.BB_ERR_WORKSPACE:
         size = C.c_size_t(0)
         _lib.check(size_of(ref, C.byref(size)), what)
-        t, ws = _take_scratch(device, stream, tickets, size.value)
+        t, ws, lock = _take_scratch(device, stream, tickets, size.value)
         a.tickets = t.data_ptr()
-        status = run(ref, ws.data_ptr(), ws.numel(), stream)
+        with lock:
+            status = run(ref, ws.data_ptr(), ws.numel(), stream)
     if status:
         _lib.check(status, what)
 
