@@ -370,11 +370,13 @@ typedef struct {
   float* out_probs;
   void* out_idx; int64_t so_i;
   int64_t splits;                         /* 0: chosen to fill the GPU */
-  int32_t* tickets; int64_t n_tickets;    /* device counters, all zero when the call runs and left zero (after a fault
-                                             of bb_device_fault: to be zeroed), or NULL. With them a call takes one
-                                             launch, without them two. bb_qkv_decode: one for every KV head and 8
-                                             query rows (H / Hkv * t rows a KV head); bb_qkv_route: two a KV head.
-                                             Calls that may overlap on the GPU need their own. */
+  int32_t* tickets; int64_t n_tickets;    /* device counters, all zero when the call runs and left zero, or NULL. With
+                                             them a call takes one launch, without them two. bb_qkv_decode: one for
+                                             every KV head and 8 query rows (H / Hkv * t rows a KV head);
+                                             bb_qkv_route: two a KV head, and a bounded wait of the CTAs of a KV head
+                                             for each other; where it runs out (code 48 of bb_device_fault) the
+                                             probabilities concerned are NaN, and the counters are left zero all the
+                                             same. Calls that may overlap on the GPU need their own. */
   float scale;
   int dtype;                              /* of q and out: BB_F16 / BB_BF16 */
   int idx_i64, out_idx_i64;

@@ -1374,19 +1374,22 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 1) qkv_scores_kernel(const A
   if constexpr (FUSED) {
     __shared__ float2 stats[Y::COLS];
     __shared__ bool all;
-    int32_t* arrived = p.tickets + 2 * kv;  // and [1]: those that have seen all arrive
+    int32_t* arrived = p.tickets + 2 * kv;  // and [1]: those that have left the wait
     __syncthreads();
     if (threadIdx.x == 0) {
       __threadfence();  // the barrier's writes before it, of all threads
       atomicAdd(arrived, 1);
       all = wait_arrivals(arrived, p.splits);
-      if (all && atomicAdd(arrived + 1, 1) == p.splits - 1) arrived[0] = arrived[1] = 0;
+      // Every CTA arrives once and then leaves once, whether or not its wait ran out, so the last to leave comes after all
+      // arrivals: the counters are zero again after every launch.
+      if (atomicAdd(arrived + 1, 1) == p.splits - 1) arrived[0] = arrived[1] = 0;
       __threadfence();
     }
     __syncthreads();
-    if (!all) return;
     if (warp < Y::COLS) {
-      const float2 v = warp < p.groups ? merged_stats(p, kv, warp, lane) : make_float2(0.f, 0.f);
+      float2 v = make_float2(0.f, 0.f);
+      if (!all) v = make_float2(NAN, NAN);  // the wait ran out: NaN in the place of this CTA's probabilities
+      else if (warp < p.groups) v = merged_stats(p, kv, warp, lane);
       if (lane == 0) stats[warp] = v;
     }
     __syncthreads();

@@ -44,8 +44,8 @@ def _stream(device):
 
 # Counters (zero between calls), a workspace and a lock, one set a stream, for calls that run one after the other on it. They
 # grow to the largest call's and stay. A call holds the lock while it enqueues: its launches hand each other results in the
-# workspace, and a call of another thread on the stream must come after the last of them. A program that goes on after a fault
-# that bb_device_fault reports clears this first: the counters may have been left above zero.
+# workspace, and a call of another thread on the stream must come after the last of them. The kernels leave the counters at
+# zero whatever happens, a routing wait that runs out (code 48 of bb_device_fault) included.
 _scratch = {}
 
 
