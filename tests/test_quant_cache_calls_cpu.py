@@ -54,3 +54,61 @@ def test_threads_on_one_stream_do_not_share_a_workspace_in_a_call(calls):
     for t in threads:
         t.join()
     assert len(calls.seen) == 5 and not shared
+
+
+@pytest.fixture
+def on_gpu_0(monkeypatch):
+    """GPU 0 is current as far as the wrappers can tell; the GPU that is current, as a list of one."""
+    current = [0]
+
+    class Enter:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Enter)
+    return current
+
+
+@pytest.mark.parametrize("index", [0, 1])
+def test_attention_calls_run_with_the_cache_s_gpu_current(on_gpu_0, monkeypatch, index):
+    at = []
+
+    def take(device, *args):
+        at.append(on_gpu_0[0])
+        return torch.zeros(8, dtype=torch.int32), torch.zeros(8, dtype=torch.uint8), threading.Lock()
+
+    def run(*args):
+        at.append(on_gpu_0[0])
+        return 0
+
+    monkeypatch.setattr(quant_cache, "_take_scratch", take)
+    quant_cache._run("call", run, None, _lib.QkvAttnArgs(), torch.device("cuda", index), 0, 4)
+    assert at == [index, index] and on_gpu_0 == [0]
+
+
+@pytest.mark.parametrize("index", [0, 1])
+def test_write_and_read_run_with_the_cache_s_gpu_current(on_gpu_0, monkeypatch, index):
+    kv = quant_cache.QuantKV(2, 10, 64, device="cpu")
+    at = []
+
+    def stop(*args, **kw):
+        at.append(on_gpu_0[0])
+        raise RuntimeError("no further")
+
+    class Rows:  # as far as write looks before it calls anything
+        device, dtype, shape = torch.device("cuda", index), torch.bfloat16, (2, 3, 64)
+
+    kv.device = torch.device("cuda", index)
+    monkeypatch.setattr(quant_cache, "_rows", stop)
+    monkeypatch.setattr(torch, "empty_strided", stop)
+    for call in (lambda: kv.write(Rows(), Rows(), 0), lambda: kv.read()):
+        with pytest.raises(RuntimeError, match="no further"):
+            call()
+    assert at == [index, index] and on_gpu_0 == [0]

@@ -9,7 +9,7 @@ values that the cache now holds, so that a prefill attends to what later steps w
 of it in between. The format and the arithmetic are described at ``bb_qkv_cache`` in
 ``include/bb_b200.h``.
 
-Everything runs on the current stream without synchronising; ``n`` and ``at`` may be 1-element GPU
+Everything runs on the current stream of the cache's device without synchronising; ``n`` and ``at`` may be 1-element GPU
 integer tensors that the kernels read at run time, so a captured CUDA graph follows a growing cache.
 """
 from __future__ import annotations
@@ -42,6 +42,11 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _elsewhere(device):
+    """Whether another GPU than ``device`` is current: a launch would go there, with this one's pointers."""
+    return device.type == "cuda" and torch._C._cuda_getDevice() != device.index
+
+
 # Counters (zero between calls), a workspace and a lock, one set a stream, for calls that run one after the other on it. They
 # grow to the largest call's and stay. A call holds the lock while it enqueues: its launches hand each other results in the
 # workspace, and a call of another thread on the stream must come after the last of them. The kernels leave the counters at
@@ -65,6 +70,9 @@ def _take_scratch(device, stream, tickets, nbytes):
 
 def _run(what, run, size_of, a, device, stream, tickets):
     """One call of a C entry that takes a workspace: with the stream's, or a larger one if that is too small."""
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return _run(what, run, size_of, a, device, stream, tickets)
     ref = C.byref(a)
     t, ws, lock = _take_scratch(device, stream, tickets, 1)
     a.tickets, a.n_tickets = t.data_ptr(), tickets
@@ -151,6 +159,9 @@ class QuantKV:
         dev = self.device
         if k.device != dev or v.device != dev or dev.type != "cuda":
             raise ValueError("QuantKV.write requires CUDA tensors on the cache's device")
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self.write(k, v, at, values=values)
         dtype = _ops._DT.get(k.dtype)
         if dtype is None or v.dtype != k.dtype:
             raise ValueError("QuantKV.write: k and v must share one of f16/bf16/f32")
@@ -190,6 +201,9 @@ class QuantKV:
             raise ValueError("QuantKV.read: dtype must be one of f16/bf16/f32")
         if dev.type != "cuda":
             raise ValueError("QuantKV.read requires a CUDA cache")
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self.read(positions, start=start, stop=stop, dtype=dtype)
         a = _lib.QkvReadArgs.from_buffer_copy(self._read)
         hk, d = self.kv_heads, self.head_dim
         if positions is None:
