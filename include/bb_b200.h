@@ -365,7 +365,7 @@ typedef struct {
   const void* idx; int64_t si_r;          /* int32, or int64 with idx_i64 */
   int64_t route_rows, route_k;            /* bb_qkv_route: route_k = keys to select */
   int64_t n; const int64_t* n_dev;
-  int64_t heads, t, front, window;
+  int64_t heads, t, front, window;        /* heads * t <= 2^30 */
   void* out; int64_t so_h, so_t;          /* [H, t, d] in the q dtype */
   float* out_probs;
   void* out_idx; int64_t so_i;

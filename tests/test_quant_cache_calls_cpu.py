@@ -112,3 +112,22 @@ def test_write_and_read_run_with_the_cache_s_gpu_current(on_gpu_0, monkeypatch, 
         with pytest.raises(RuntimeError, match="no further"):
             call()
     assert at == [index, index] and on_gpu_0 == [0]
+
+
+def test_the_number_of_query_rows_is_bounded_by_32_bits_only():
+    """Follow-up prompts: 32 heads x 4096 tokens and more are planned; the workspace holds no partial results where the
+    query rows fill the GPU without cutting the keys."""
+    import ctypes as C
+
+    from test_quant_cache_cpu import BUF, attn
+    L, size = _lib.lib(), C.c_size_t(0)
+    big = dict(k_codes_h=64 * 2 ** 21, k_meta_h=4 * 2 ** 21, v_codes_h=64 * 2 ** 21, v_meta_h=4 * 2 ** 21, cap=2 ** 21)
+    for t in (2047, 2048, 4096, 131072, 2 ** 25):
+        a = attn(big, n=2 ** 21, t=t, window=2 ** 21, front=0)
+        assert L.bb_qkv_decode_workspace_size(C.byref(a), C.byref(size)) == 0, t
+        assert 0 < size.value <= 1 << 20, (t, size.value)
+    a = attn(big, n=2 ** 21, t=2 ** 25 + 1, window=2 ** 21)
+    assert L.bb_qkv_decode_workspace_size(C.byref(a), C.byref(size)) == 2 and "tokens" in L.bb_last_error().decode()
+    a = attn(big, n=2 ** 21, t=2 ** 25, window=2 ** 21, splits=1000)   # no more CTAs than a grid has
+    assert L.bb_qkv_decode_workspace_size(C.byref(a), C.byref(size)) == 0
+    assert a.cache.k_codes == BUF

@@ -1473,8 +1473,8 @@ int check_attn(const bb_qkv_attn_args* a, const char* what, bool need_v) {
   if (a->heads <= 0 || a->heads % a->cache.kv_heads || a->heads > 65535)
     return fail(BB_ERR_SHAPE, "%s: heads must be a positive multiple of kv_heads (at most 65535)", what);
   if (a->heads / a->cache.kv_heads > 1024) return fail(BB_ERR_UNSUPPORTED, "%s: at most 1024 query heads a KV head", what);
-  if (a->t <= 0 || a->t > 65535 || a->t * a->heads > (int64_t)65535)
-    return fail(BB_ERR_SHAPE, "%s: heads * tokens must lie in [1, 65535]", what);
+  if (a->t <= 0 || a->t > ((int64_t)1 << 30) / a->heads)  // query rows are counted in 32 bits
+    return fail(BB_ERR_SHAPE, "%s: heads * tokens must lie in [1, 2^30]", what);
   if (a->n < 0 || a->n > a->cache.cap) return fail(BB_ERR_ARG, "%s: n must lie in [0, capacity]", what);
   if (a->front < 0 || a->window < 0) return fail(BB_ERR_ARG, "%s: front and window must be >= 0", what);
   if (a->route_k < 0) return fail(BB_ERR_ARG, "%s: bad route count", what);
@@ -1490,7 +1490,7 @@ void plan_grid(const bb_qkv_attn_args* a, int64_t steps, bool decode, AttnPlan* 
   pl->ztiles = cdiv(pl->cols, (int64_t)pl->columns);
   const int64_t w = !decode ? SCORE_WARPS : (pl->columns == 8 || a->cache.bits == 8 ? warps<8, true>() : warps<4, true>());
   const int64_t s = a->splits > 0 ? a->splits : std::max<int64_t>(1, (int64_t)num_sms() / (a->cache.kv_heads * pl->ztiles));
-  pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(steps, w), (int64_t)1024}));
+  pl->splits = std::max<int64_t>(1, std::min<int64_t>({s, cdiv(steps, w), (int64_t)1024, INT32_MAX / pl->ztiles}));
 }
 
 int plan_decode(const bb_qkv_attn_args* a, AttnPlan* pl) {
@@ -1505,10 +1505,11 @@ int plan_decode(const bb_qkv_attn_args* a, AttnPlan* pl) {
   const int64_t lists = a->route_k > 0 && a->route_rows != a->cache.kv_heads ? a->heads / a->cache.kv_heads : 1;
   if (a->route_k > ((int64_t)1 << 27) / lists) return fail(BB_ERR_UNSUPPORTED, "qkv_decode: too many routed keys");
   plan_grid(a, cdiv(f, (int64_t)32) + cdiv(w, (int64_t)32) + lists * cdiv(a->route_k, (int64_t)32), true, pl);
-  const int64_t rows = a->cache.kv_heads * pl->ztiles * pl->columns * pl->splits;
+  // partial results, of which a single split has none
+  const int64_t rows = pl->splits == 1 ? 0 : a->cache.kv_heads * pl->ztiles * pl->columns * pl->splits;
   pl->ml_bytes = align_up((size_t)rows * 8, 256);
   pl->acc_bytes = align_up((size_t)(rows * a->cache.d) * 4, 256);
-  pl->total = pl->ml_bytes + pl->acc_bytes;
+  pl->total = std::max<size_t>(pl->ml_bytes + pl->acc_bytes, 256);
   return BB_OK;
 }
 
