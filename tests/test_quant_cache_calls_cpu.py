@@ -131,3 +131,30 @@ def test_the_number_of_query_rows_is_bounded_by_32_bits_only():
     a = attn(big, n=2 ** 21, t=2 ** 25, window=2 ** 21, splits=1000)   # no more CTAs than a grid has
     assert L.bb_qkv_decode_workspace_size(C.byref(a), C.byref(size)) == 0
     assert a.cache.k_codes == BUF
+
+
+def test_kept_buffers_stay_whatever_the_calls_need(calls):
+    """Calls of other sizes in between do not replace a stream's buffers, and a call too large for them gets its own."""
+    calls()
+    first = calls.seen[-1]
+    for kw in (dict(need=100 << 20), dict(tickets=2000), dict(need=100 << 20), dict(tickets=70000, need=50 << 20)):
+        calls(**kw)
+        ws, nbytes, tickets, n_tickets = calls.seen[-1]
+        assert nbytes >= kw.get("need", 0) and 0 < n_tickets <= kw.get("tickets", 16)
+        calls()
+        assert calls.seen[-1] == first
+    assert len(quant_cache._scratch) == 1
+    kept = sum(x.numel() * x.element_size() for s in quant_cache._scratch.values() for x in s if isinstance(x, torch.Tensor))
+    assert kept <= 16 << 20
+
+
+def test_a_captured_call_fills_its_counters_once(calls, monkeypatch):
+    """Every fill under a capture is a node that each replay pays for. A captured call uses nothing of the kept buffers."""
+    calls()
+    filled, zeros = [], torch.zeros
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(torch, "zeros", lambda *a, **kw: filled.append(zeros(*a, **kw)) or filled[-1])
+    for need in (1000, 100 << 20):
+        calls(need=need)
+        assert len(filled) == 1 and calls.seen[-1][2] == filled.pop().data_ptr()
+        assert calls.seen[-1][0] != calls.seen[0][0] and calls.seen[-1][2] != calls.seen[0][2]

@@ -47,42 +47,43 @@ def _elsewhere(device):
     return device.type == "cuda" and torch._C._cuda_getDevice() != device.index
 
 
-# Counters (zero between calls), a workspace and a lock, one set a stream, for calls that run one after the other on it. They
-# grow to the largest call's and stay. A call holds the lock while it enqueues: its launches hand each other results in the
+# Counters (zero between calls), a workspace and a lock, one set a stream, for calls that run one after the other on it. Their
+# sizes are fixed: a call that needs a larger workspace (a routing over some 64K keys or more, which takes far longer than the
+# allocation) has its own, and a call that needs more counters (only with explicit splits) takes two launches instead of
+# one. A call holds the lock while it enqueues: its launches hand each other results in the
 # workspace, and a call of another thread on the stream must come after the last of them. The kernels leave the counters at
 # zero whatever happens, a routing wait that runs out (code 48 of bb_device_fault) included.
 _scratch = {}
+_TICKETS, _WORKSPACE = 1024, 8 << 20
 
 
-def _take_scratch(device, stream, tickets, nbytes):
-    """Tickets and a workspace of at least these sizes for a call on ``stream``, and the lock under which to use them. Calls
-    under a graph capture get their own, which the graph zeroes and keeps."""
+def _take_scratch(device, stream):
+    """Tickets, a workspace and the lock under which to use them, for a call on ``stream``. Calls under a graph capture get
+    their own, which the graph zeroes and keeps."""
     if torch.cuda.is_current_stream_capturing():
-        return (torch.zeros(tickets, dtype=torch.int32, device=device),
-                torch.empty(nbytes, dtype=torch.uint8, device=device), threading.Lock())
+        return (torch.zeros(_TICKETS, dtype=torch.int32, device=device),
+                torch.empty(1, dtype=torch.uint8, device=device), threading.Lock())
     s = _scratch.get((device.index, stream))
-    if s is None or s[0].numel() < tickets or s[1].numel() < nbytes:
-        s = _scratch[device.index, stream] = (torch.zeros(max(tickets, 1024), dtype=torch.int32, device=device),
-                                              torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device),
-                                              threading.Lock())
+    if s is None:
+        s = _scratch[device.index, stream] = (torch.zeros(_TICKETS, dtype=torch.int32, device=device),
+                                              torch.empty(_WORKSPACE, dtype=torch.uint8, device=device), threading.Lock())
     return s
 
 
 def _run(what, run, size_of, a, device, stream, tickets):
-    """One call of a C entry that takes a workspace: with the stream's, or a larger one if that is too small."""
+    """One call of a C entry that takes a workspace: with the stream's, or one of its own if that is too small."""
     if _elsewhere(device):
         with torch.cuda.device(device):
             return _run(what, run, size_of, a, device, stream, tickets)
     ref = C.byref(a)
-    t, ws, lock = _take_scratch(device, stream, tickets, 1)
-    a.tickets, a.n_tickets = t.data_ptr(), tickets
+    t, ws, lock = _take_scratch(device, stream)
+    a.tickets, a.n_tickets = t.data_ptr(), min(tickets, _TICKETS)
     with lock:
         status = run(ref, ws.data_ptr(), ws.numel(), stream)
     if status == _lib.BB_ERR_WORKSPACE:
         size = C.c_size_t(0)
         _lib.check(size_of(ref, C.byref(size)), what)
-        t, ws, lock = _take_scratch(device, stream, tickets, size.value)
-        a.tickets = t.data_ptr()
+        ws = torch.empty(size.value, dtype=torch.uint8, device=device)
         with lock:
             status = run(ref, ws.data_ptr(), ws.numel(), stream)
     if status:
