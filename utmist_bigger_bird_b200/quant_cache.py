@@ -31,9 +31,10 @@ def _rows(x):
     sh, st, sd = x.stride()
     p, es = x.data_ptr(), x.element_size()
     if sd != 1 or (p | sh * es | st * es) & 15:
-        x = x.contiguous()
-        sh, st, _ = x.stride()
-        p = x.data_ptr()
+        # not contiguous(), which hands back what only an address or the stride of a single head or row is wrong with
+        x = x.clone(memory_format=torch.contiguous_format)
+        p, st = x.data_ptr(), x.shape[2]
+        sh = x.shape[1] * st
     return x, p, sh, st
 
 
