@@ -34,3 +34,18 @@ def test_rows_that_need_no_copy_are_not_copied():
     for x in (flat(2 * 3 * 64).view(2, 3, 64), flat(2 * 3 * 64).view(3, 2, 64).transpose(0, 1),
               flat(2 * 3 * 136).view(2, 3, 136)[..., 8:72]):
         assert _rows(x)[1] == x.data_ptr()
+
+
+@pytest.mark.parametrize("which", [1, 3])
+def test_pairs_at_an_odd_head_stride_are_refused(which):
+    """(step, low) pairs are addressed as 32-bit words: heads an odd number of elements apart cannot be."""
+    def buffers(stride, hk=2):
+        b = [torch.zeros(hk, 10, 32, dtype=torch.uint8), torch.zeros(hk, 10, 1, 2, dtype=torch.bfloat16),
+             torch.zeros(hk, 10, 32, dtype=torch.uint8), torch.zeros(hk, 10, 1, 2, dtype=torch.bfloat16)]
+        b[which] = torch.zeros(64, dtype=torch.bfloat16).as_strided((hk, 10, 1, 2), (stride, 2, 2, 1))
+        return b
+    with pytest.raises(ValueError, match="pairs"):
+        QuantKV.from_buffers(*buffers(21), bits=4)
+    for kv in (QuantKV.from_buffers(*buffers(22), bits=4), QuantKV.from_buffers(*buffers(21, 1), bits=4)):
+        assert kv.group == 64
+    assert QuantKV.from_buffers(*buffers(22), bits=4)._struct.k_meta_h in (10, 11)

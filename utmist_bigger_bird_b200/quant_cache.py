@@ -124,6 +124,8 @@ class QuantKV:
                 raise ValueError("QuantKV: codes and meta do not match")
             if codes.stride()[1:] != (codes.shape[2], 1) or meta.stride()[1:] != (2 * meta.shape[2], 2, 1):
                 raise ValueError("QuantKV: rows must be dense")
+            if codes.shape[0] > 1 and meta.stride(0) % 2:
+                raise ValueError("QuantKV: heads of meta must be whole (step, low) pairs apart")
         if k_codes.shape != v_codes.shape or k_meta.shape != v_meta.shape:
             raise ValueError("QuantKV: keys and values do not match")
         if any(t.device != k_codes.device for t in (k_meta, v_codes, v_meta)):
