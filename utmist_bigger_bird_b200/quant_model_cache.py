@@ -13,6 +13,8 @@ cache longer than front + window + k_route, ``quant_route`` and ``quant_decode``
 """
 from __future__ import annotations
 
+import torch
+
 from .quant_cache import QuantKV, quant_decode, quant_route
 
 __all__ = ["make_quant_cache"]
@@ -50,6 +52,7 @@ def _layer_class():
 
         def __init__(self, kv, sparse):
             self.kv, self.sparse, self.length, self._kept = kv, sparse, 0, None
+            self.dtype = torch.bfloat16  # of keys and values as tensors: the model's, once rows have come
             self.is_initialized = True
 
         def lazy_initialization(self, key_states, value_states):
@@ -59,6 +62,7 @@ def _layer_class():
             if key_states.shape[0] != 1:
                 raise ValueError("batch size 1 only")
             first, t = self.length == 0, key_states.shape[-2]
+            self.dtype = key_states.dtype
             values = self.kv.write(key_states[0], value_states[0], self.length, values=first)
             self.length += t
             if first:
@@ -69,7 +73,7 @@ def _layer_class():
         # RDAttention.evict sets keys, then values, to the rows that stay
         @property
         def keys(self):
-            return self.kv.read(stop=self.length)[0][None]
+            return self.kv.read(stop=self.length, dtype=self.dtype)[0][None]
 
         @keys.setter
         def keys(self, rows):
@@ -77,7 +81,7 @@ def _layer_class():
 
         @property
         def values(self):
-            return self.kv.read(stop=self.length)[1][None]
+            return self.kv.read(stop=self.length, dtype=self.dtype)[1][None]
 
         @values.setter
         def values(self, rows):
