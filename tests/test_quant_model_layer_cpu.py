@@ -41,3 +41,16 @@ def test_keys_and_values_have_the_model_s_type(dtype):
     assert torch.equal(x.keys, k) and torch.equal(x.values, v)      # no bits lost on the way
     x.keys, x.values = k[:, :, :3], v[:, :, :3]                     # eviction
     assert x.length == 3 and torch.equal(x.keys, k[:, :, :3]) and x.values.dtype == dtype
+
+
+def test_what_a_step_cannot_attend_to_is_refused_before_it_is_written():
+    """fp32 queries are not attended to over codes: the layer says so while its rows and length are as they were."""
+    x = layer(torch.float32)
+    k = torch.ones(1, 2, 5, 64)
+    x.update(k, k)                                                  # a prompt's attention is the model's own
+    rows = [r.clone() for r in x.kv.rows]
+    with pytest.raises(ValueError, match="FP16/BF16"):
+        x.update(2 * k[:, :, :1], 2 * k[:, :, :1])
+    assert x.length == 5 and all(torch.equal(a, b) for a, b in zip(rows, x.kv.rows))
+    x.update(k[:, :, :1].half(), k[:, :, :1].half())
+    assert x.length == 6

@@ -9,7 +9,8 @@ cache, for models whose attention is ``RDAttention`` (``install``).
 stand for, so the prefill attends to what later steps read; later calls return a handle whose ``attend``
 ``RDAttention.exact_attention`` calls: dense attention over the cache, or, for single tokens with ``sparse`` and a
 cache longer than front + window + k_route, ``quant_route`` and ``quant_decode`` over front | window | routes.
-``RDAttention(kv_evict=True)`` works: the kept rows are quantised again in the place of the prompt.
+Steps after the prompt require FP16 or BF16. ``RDAttention(kv_evict=True)`` works: the kept rows are quantised again in
+the place of the prompt.
 """
 from __future__ import annotations
 
@@ -62,6 +63,8 @@ def _layer_class():
             if key_states.shape[0] != 1:
                 raise ValueError("batch size 1 only")
             first, t = self.length == 0, key_states.shape[-2]
+            if not first and key_states.dtype not in (torch.float16, torch.bfloat16):  # before any row is written
+                raise ValueError("attention over a quantised cache requires FP16/BF16")
             self.dtype = key_states.dtype
             values = self.kv.write(key_states[0], value_states[0], self.length, values=first)
             self.length += t
