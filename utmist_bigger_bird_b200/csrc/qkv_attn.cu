@@ -370,7 +370,8 @@ __device__ __forceinline__ void mma_h0(float (&d)[4], const uint32_t (&a)[4], co
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
 
-// C += ones B over 8 of k: rows 0-7 (half 0) or 8-15 (half 1) of C take the column sums of B.
+// C += ones B over 8 of k: rows 0-7 (half 0) or 8-15 (half 1) of C take the column sums of B. The other half's rows are
+// multiplied by zero, so where two groups share C, B must not be NaN (unless it is for every group: see scaled_step).
 __device__ __forceinline__ void mma_sum(float (&d)[4], int half, uint32_t b) {
   constexpr uint32_t ONES = 0x3C003C00u;  // fp16 1, 1
   asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
@@ -697,6 +698,13 @@ template <bool SPLIT> struct Running {
 template <int BITS> constexpr float CENTRE = BITS == 4 ? 8.f : 128.f;
 constexpr int SETTLE = 4;               // steps between two subtractions
 
+// A step in units of P. Where several groups' sums of P share accumulators, a group that is stored as NaN counts as zero here: its
+// dimensions become NaN by `mid`, which is per group. (max.f32 returns the operand that is a number.)
+template <bool SHARED> __device__ __forceinline__ float scaled_step(float step, float pscale) {
+  const float t = step * pscale;
+  return SHARED ? fmaxf(t, 0.f) : t;
+}
+
 // What a power of two the codes of accumulator tile t carry: 2^-24, with 4 bits 2^-20 in the second tile.
 template <int BITS> __device__ __forceinline__ constexpr float code_unit(int t) {
   return BITS == 4 && t == 1 ? 9.5367431640625e-07f : 5.9604644775390625e-08f;
@@ -757,7 +765,7 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
       for (int gi = 0; gi < NG; ++gi) {
         const float s0 = step_of(m0[gi]), s1 = step_of(m1[gi]);
         const float h0 = fmaf(CENTRE<BITS>, s0, low_of(m0[gi])), h1 = fmaf(CENTRE<BITS>, s1, low_of(m1[gi]));
-        const float t0 = s0 * run.pscale, t1 = s1 * run.pscale;
+        const float t0 = scaled_step<(NG > 1)>(s0, run.pscale), t1 = scaled_step<(NG > 1)>(s1, run.pscale);
         float u[4] = {e[x][0] * t0, e[x][1] * t0, e[x][2] * t1, e[x][3] * t1};
         if constexpr (EDGE) {  // rows that do not count may hold NaN
           float z[4] = {e[x][0] * h0, e[x][1] * h0, e[x][2] * h1, e[x][3] * h1};
@@ -920,7 +928,8 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true> {
 #pragma unroll
         for (int j = 0; j < NU; ++j) {
           const uint32_t mm = m[2 * x + half][j];
-          const float sj = step_of(mm), hj = fmaf(CENTRE<BITS>, sj, low_of(mm)), tj = sj * run.pscale;
+          const float sj = step_of(mm), hj = fmaf(CENTRE<BITS>, sj, low_of(mm));
+          const float tj = scaled_step<(NU > 1)>(sj, run.pscale);
           float u[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
