@@ -45,11 +45,7 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
+using qkv::max_nan;
 
 // The bf16 numbers next to x: not above it; not below it (x >= 0). As fp32 bit patterns, whose upper
 // halves are the bf16 numbers.

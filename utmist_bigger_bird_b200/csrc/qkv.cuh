@@ -9,6 +9,13 @@ namespace qkv {
 
 constexpr int K_RUN = 8, V_RUN = 4;  // consecutive dimensions that stay together in a row's order
 
+// NaN if either is (fmaxf returns the other).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Checks of the cache's description; `what` opens the message.

@@ -17,10 +17,13 @@
 // code 2^-24 (code 2^-20), a subnormal that the tensor cores take as it is, so a masked word is a pair of
 // operands. The powers of two are undone in fp32. Keys (rows of K) and dimensions (rows of V transposed)
 // are the 16 rows of a product and the query rows its 8 columns (Layout, Accum).
-//   q: fp16 after a power of two that brings the row's largest element to [2^14, 2^15) (exact for bf16
-// and fp16 queries, except elements below 2^-28 of the largest, which lose relative precision only).
-//   p s: rounded to fp16 once, scaled by powers of two (a running bound of the steps, the running
-// maximum of the scores) to at most 2^15, so that p down to 2^-29 of the largest keeps all 11 bits.
+//   q: fp16 after a power of two that brings the row's largest element to [2^14, 2^15), against 4-bit codes that
+// carry 2^-20 to [2^10, 2^11) (exact for bf16 and fp16 queries, except elements below 2^-28, there 2^-24, of the
+// largest, which lose relative precision only).
+//   P = p s: rounded to fp16 once, in units in which p = 1 and s = the group's bound make 2^11. The bound is a power of
+// two, at most twice the largest step of the group that the warp has met; p refers to the running maximum, which may lag
+// by 2^4. So P <= 2^15; it keeps all 11 bits while p s is at least 2^-24 of the group's largest step, and is off by at most
+// 2^-36 of the bound below that.
 // Scores, exponentials, sums and accumulators are fp32.
 //
 // What bounds it: bytes, 2 (d bits / 8 + 4 d / group) a key and KV head, and close behind them the issue slots that unpack
@@ -304,6 +307,11 @@ template <int N> __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uin
     for (int i = 0; i < N; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + i * 4));
   }
 }
+__device__ __forceinline__ uint32_t lds_word(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
 __device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
   uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
@@ -371,7 +379,7 @@ __device__ __forceinline__ void mma_h0(float (&d)[4], const uint32_t (&a)[4], co
 }
 
 // C += ones B over 8 of k: rows 0-7 (half 0) or 8-15 (half 1) of C take the column sums of B. The other half's rows are
-// multiplied by zero, so where two groups share C, B must not be NaN (unless it is for every group: see scaled_step).
+// multiplied by zero, so where two groups share C, a group's B is NaN only if the key's p is (for every group: see no_nan).
 __device__ __forceinline__ void mma_sum(float (&d)[4], int half, uint32_t b) {
   constexpr uint32_t ONES = 0x3C003C00u;  // fp16 1, 1
   asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
@@ -605,12 +613,42 @@ template <int BITS, int G, int NG, bool SPLIT> size_t partial_smem(int splits) {
   return std::max({ring, merge, last});
 }
 
+// A (step, low) pair with a step of zero where it is NaN: its P is zero, and the dimensions of its group become NaN by the low
+// value, in `mid`, which is per group.
+__device__ __forceinline__ uint32_t no_nan(uint32_t m) { return step_of(m) == step_of(m) ? m : m & 0xFFFF0000u; }
+
+// The steps of a group in four staged rows 8 apart, the first pair at `at`: the largest, NaN where one is.
+template <int META> __device__ __forceinline__ float largest_step(uint32_t at) {
+  float top = step_of(lds_word(at));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) top = qkv::max_nan(top, step_of(lds_word(at + i * 8 * META)));
+  return top;
+}
+// The largest of all rows' steps of the group (`top`: largest_step of this thread's rows), after NaN has been taken out of the
+// staged pairs. Threads whose lanes differ in bits 2-4 watch one group's rows between them.
+template <int META> __device__ __forceinline__ float clean_largest_step(uint32_t at, float top) {
+  if (__any_sync(0xffffffffu, top != top)) {
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t pair = at + i * 8 * META, m = no_nan(lds_word(pair));
+      top = fmaxf(top, step_of(m));
+      __syncwarp();  // threads that share the pair have read it
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(pair), "r"(m) : "memory");
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int off = 4; off < 32; off *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  return top;
+}
+
 // The softmax of a warp's columns: reference points that move only when a score exceeds them by 2^LAZY or a step
-// exceeds its bound, and the sum of p over this thread's keys.
-template <bool SPLIT> struct Running {
+// exceeds its group's bound (or is NaN), and the sum of p over this thread's keys. NB: groups that this thread's columns meet.
+template <bool SPLIT, int NB> struct Running {
   using Y = Layout<SPLIT>;
   float m[2], l[2];
-  float bound, pscale;  // a power of two above every step so far (2^-100: none); P_SCALE / bound
+  float pscale[NB];  // P_SCALE over a power of two above every step of the group so far (2^-100: none)
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -618,18 +656,29 @@ template <bool SPLIT> struct Running {
       m[k] = M_NONE;
       l[k] = 0.f;
     }
-    bound = 7.8886090522101181e-31f;
-    pscale = P_SCALE / bound;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) pscale[j] = P_SCALE * 1.2676506002282294e+30f;
+  }
+  // Powers of two: their quotients by their exponents. P_SCALE = 2^11.
+  static __device__ __forceinline__ int field(float x) { return (int)(__float_as_uint(x) >> 23); }  // x >= 0
+  static __device__ __forceinline__ float power(int field) { return __uint_as_float((uint32_t)field << 23); }
+  __device__ __forceinline__ float bound(int j) const { return power(127 + 11 + 127 - field(pscale[j])); }
+  // Raises group j's bound above `top`, where it is not yet. What the sums of P are to be multiplied by.
+  __device__ __forceinline__ float raise(int j, float top) {
+    if (!(top * pscale[j] > P_SCALE)) return 1.f;
+    const int next = 127 + 11 + 127 - (field(top) + 1), before = field(pscale[j]);
+    pscale[j] = power(next);
+    return power(max(0, 127 + next - before));
   }
 
-  // Scores s (before their factors) -> p in e. Returns whether the references moved: everything kept in units of
-  // p is then to be multiplied by f, and P.V by shrink as well.
-  template <bool EDGE>
+  // Scores s (before their factors) -> p in e. `move`: a step of this thread's rows exceeds its group's bound or is NaN; steps()
+  // then raises the bounds. Returns whether the references moved: everything kept in units of p is then to be multiplied by
+  // f, and P.V by its group's shrink as well.
+  template <bool EDGE, typename Raise>
   __device__ __forceinline__ bool update(float (&e)[Y::TILES][4], const float (&s)[Y::TILES][4],
-                                         const float (&mul)[2], const Mask<SPLIT>& mask, float smax,
-                                         float (&f)[2], float& shrink) {
+                                         const float (&mul)[2], const Mask<SPLIT>& mask, bool move, Raise steps,
+                                         float (&f)[2]) {
     constexpr int X = Y::TILES;
-    bool move = smax > bound;
 #pragma unroll
     for (int x = 0; x < X; ++x)
 #pragma unroll
@@ -641,14 +690,7 @@ template <bool SPLIT> struct Running {
     for (int x = 0; x < X; ++x) move |= fmaxf(fmax3(e[x][0], e[x][1], e[x][2]), e[x][3]) > LAZY;
     const bool moved = __any_sync(0xffffffffu, move);
     if (moved) {
-      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)));
-      shrink = 1.f;
-      if (top > bound) {
-        const float next = __uint_as_float((__float_as_uint(top) & 0x7F800000u) + 0x00800000u);
-        shrink = bound / next;
-        bound = next;
-        pscale = P_SCALE / next;
-      }
+      steps();
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         float v = -INFINITY;
@@ -698,13 +740,6 @@ template <bool SPLIT> struct Running {
 template <int BITS> constexpr float CENTRE = BITS == 4 ? 8.f : 128.f;
 constexpr int SETTLE = 4;               // steps between two subtractions
 
-// A step in units of P. Where several groups' sums of P share accumulators, a group that is stored as NaN counts as zero here: its
-// dimensions become NaN by `mid`, which is per group. (max.f32 returns the operand that is a number.)
-template <bool SHARED> __device__ __forceinline__ float scaled_step(float step, float pscale) {
-  const float t = step * pscale;
-  return SHARED ? fmaxf(t, 0.f) : t;
-}
-
 // What a power of two the codes of accumulator tile t carry: 2^-24, with 4 bits 2^-20 in the second tile.
 template <int BITS> __device__ __forceinline__ constexpr float code_unit(int t) {
   return BITS == 4 && t == 1 ? 9.5367431640625e-07f : 5.9604644775390625e-08f;
@@ -718,7 +753,7 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
   float o[G][2][4];            // block of 32 dimensions, tile of 16
   float ps[(NG + 1) / 2][4];   // sum P of groups 2i (rows 0-7) and 2i + 1 (rows 8-15)
   float mid[NG][2];            // sum p (low + C step) of this thread's keys
-  Running<SPLIT> run;
+  Running<SPLIT, NG> run;
 
   __device__ __forceinline__ void clear(int) {
     run.clear();
@@ -736,25 +771,30 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
   __device__ __forceinline__ void step(const Query<BITS, G, NG, SPLIT>& q, uint32_t st, int lane,
                                        const Mask<SPLIT>& mask) {
     const int r = lane / 4, c = lane % 4;
-    float s[2][4], e[2][4], f[2], shrink;
+    float s[2][4], e[2][4], f[2], shrink[NG];
     step_scores<BITS, G, NG, SPLIT>(q, st, st + S::KM, lane, s);
-    float smax = 0.f;
+    // The four threads that share rows r watch a group each (all of them the only one).
+    const uint32_t watch = st + S::VM + r * S::META + min(c, NG - 1) * 4;
+    const float top = largest_step<S::META>(watch);
+    float mine = run.pscale[0];  // of the group that this thread watches
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t m[NG];
-      lds_words(m, st + S::VM + (i * 8 + r) * S::META);
+    for (int gi = 1; gi < NG; ++gi) mine = c >= gi ? run.pscale[gi] : mine;
+    const auto steps = [&] {
+      const float all = clean_largest_step<S::META>(watch, top);
 #pragma unroll
-      for (int gi = 0; gi < NG; ++gi) smax = fmaxf(smax, step_of(m[gi]));  // NaN ignored
-    }
-    if (run.template update<EDGE>(e, s, q.mul, mask, smax, f, shrink)) {
+      for (int gi = 0; gi < NG; ++gi) shrink[gi] = run.raise(gi, __shfl_sync(0xffffffffu, all, gi));
+    };
+    if (run.template update<EDGE>(e, s, q.mul, mask, !(top * mine <= P_SCALE), steps, f)) {
 #pragma unroll
       for (int i = 0; i < NG * 2; ++i) mid[i / 2][i % 2] *= f[i % 2];
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[g][i / 4][i % 4] *= f[i & 1] * shrink;
+        for (int i = 0; i < 8; ++i) o[g][i / 4][i % 4] *= f[i & 1] * shrink[g / (G / NG)];
 #pragma unroll
-      for (int i = 0; i < (NG + 1) / 2 * 4; ++i) ps[i / 4][i % 4] *= f[i & 1] * shrink;
+      for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) ps[gi / 2][gi % 2 * 2 + k] *= f[k] * shrink[gi];
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -765,7 +805,7 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
       for (int gi = 0; gi < NG; ++gi) {
         const float s0 = step_of(m0[gi]), s1 = step_of(m1[gi]);
         const float h0 = fmaf(CENTRE<BITS>, s0, low_of(m0[gi])), h1 = fmaf(CENTRE<BITS>, s1, low_of(m1[gi]));
-        const float t0 = scaled_step<(NG > 1)>(s0, run.pscale), t1 = scaled_step<(NG > 1)>(s1, run.pscale);
+        const float t0 = s0 * run.pscale[gi], t1 = s1 * run.pscale[gi];
         float u[4] = {e[x][0] * t0, e[x][1] * t0, e[x][2] * t1, e[x][3] * t1};
         if constexpr (EDGE) {  // rows that do not count may hold NaN
           float z[4] = {e[x][0] * h0, e[x][1] * h0, e[x][2] * h1, e[x][3] * h1};
@@ -847,7 +887,7 @@ template <int BITS, int G, int NG, bool SPLIT> struct Accum {
 #pragma unroll
           for (int h = 0; h < 2; ++h)  // 4 bits: tile t holds dimensions 4r + t, 4r + t + 2; 8 bits: 4r + 2t, + 1
             put(Y::col(c, k), g * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
-                fmaf(o[g][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound, mid[g / (G / NG)][k]));
+                fmaf(o[g][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound(g / (G / NG)), mid[g / (G / NG)][k]));
     }
   }
 };
@@ -865,7 +905,7 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true> {
   float o[PAIRS][2][4];
   float ps[4];                     // sum P of this thread's groups 0 (rows 0-7) and 1 (rows 8-15)
   float mid[NU][2];
-  Running<true> run;
+  Running<true, NU> run;
   uint32_t sel0, sel1;             // place the first / second 16 bits of a word in this column's half
 
   __device__ __forceinline__ void clear(int lane) {
@@ -883,30 +923,27 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true> {
   template <bool EDGE>
   __device__ __forceinline__ void step(const Query<BITS, G, NG, true>& q, uint32_t st, int lane, const Mask<true>& mask) {
     const int r = lane / 4, c = lane % 4;
-    float s[1][4], e[1][4], f[2], shrink;
+    float s[1][4], e[1][4], f[2], shrink[NU];
     step_scores<BITS, G, NG, true>(q, st, st + S::KM, lane, s);
-    // (step, low) of this thread's groups: rows r and r + 8 of both tiles
-    uint32_t m[4][NU];
-    float smax = 0.f;
+    // (step, low) of this thread's group j in row r: pairs + j * PAIR; rows lie 8 apart.
+    constexpr int PAIR = NG == G ? 8 : 4;
+    const uint32_t pairs = st + S::VM + r * S::META + (NG == G ? (c >> 1) * 4 : 0);
+    // Threads c and c ^ 1, whose pairs are the same, watch a group each (both the only one).
+    const uint32_t watch = pairs + (NU > 1 ? (c & 1) * PAIR : 0);
+    const float top = largest_step<S::META>(watch);
+    const float mine = NU > 1 && (c & 1) ? run.pscale[NU - 1] : run.pscale[0];
+    const auto steps = [&] {
+      const float all = clean_largest_step<S::META>(watch, top);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t at = st + S::VM + (i * 8 + r) * S::META;
-      if constexpr (NG == G) {
-#pragma unroll
-        for (int j = 0; j < NU; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(m[i][j]) : "r"(at + j * 8 + (c >> 1) * 4));
-      } else {
-        lds_words(m[i], at);
-      }
-#pragma unroll
-      for (int j = 0; j < NU; ++j) smax = fmaxf(smax, step_of(m[i][j]));  // NaN ignored
-    }
-    if (run.template update<EDGE>(e, s, q.mul, mask, smax, f, shrink)) {
+      for (int j = 0; j < NU; ++j) shrink[j] = run.raise(j, __shfl_sync(0xffffffffu, all, NU > 1 ? (c & 2) | j : c));
+    };
+    if (run.template update<EDGE>(e, s, q.mul, mask, !(top * mine <= P_SCALE), steps, f)) {
 #pragma unroll
       for (int i = 0; i < NU * 2; ++i) mid[i / 2][i % 2] *= f[i % 2];
 #pragma unroll
-      for (int i = 0; i < PAIRS * 8; ++i) o[i / 8][i / 4 % 2][i % 4] *= f[i & 1] * shrink;
+      for (int i = 0; i < PAIRS * 8; ++i) o[i / 8][i / 4 % 2][i % 4] *= f[i & 1] * shrink[NU == PAIRS ? i / 8 : 0];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ps[i] *= f[i & 1] * shrink;
+      for (int i = 0; i < NU * 2; ++i) ps[i] *= f[i & 1] * shrink[i / 2];
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -927,9 +964,8 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true> {
         uint32_t b[NU][2];
 #pragma unroll
         for (int j = 0; j < NU; ++j) {
-          const uint32_t mm = m[2 * x + half][j];
-          const float sj = step_of(mm), hj = fmaf(CENTRE<BITS>, sj, low_of(mm));
-          const float tj = scaled_step<(NU > 1)>(sj, run.pscale);
+          const uint32_t mm = lds_word(pairs + (2 * x + half) * 8 * S::META + j * PAIR);
+          const float sj = step_of(mm), hj = fmaf(CENTRE<BITS>, sj, low_of(mm)), tj = sj * run.pscale[j];
           float u[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
@@ -1001,7 +1037,8 @@ template <int BITS, int G, int NG> struct Accum<BITS, G, NG, true> {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             put(Y::col(c, k), (2 * i + (c >> 1)) * 32 + 4 * r + (BITS == 4 ? t + 2 * h : 2 * t + h),
-                fmaf(o[i][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound, mid[NU == PAIRS ? i : 0][k]));
+                fmaf(o[i][t][2 * h + k] * (1.f / (P_SCALE * code_unit<BITS>(t))), run.bound(NU == PAIRS ? i : 0),
+                     mid[NU == PAIRS ? i : 0][k]));
     }
   }
 };
