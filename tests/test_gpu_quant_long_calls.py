@@ -41,3 +41,18 @@ def test_a_model_s_long_follow_up():
         want = torch.cat([run(two, 300, 800), run(two, 800, 1400)], 1)
     close(got, want)
     assert [layer.length for layer in one.layers] == [1400, 1400]
+
+
+def test_explicit_splits_with_more_tiles_than_counters():
+    """More tiles of query rows than a stream keeps counters for: the splits are merged in a second launch."""
+    from utmist_bigger_bird_b200 import _lib
+    hk, g, t, n, d = 2, 64, 200, 900, 64                     # 2 x 1600 tiles
+    kv, kval, vval, wval = filled(hk, 1000, d, 4, 32)
+    q = rand((hk * g, t, d), 51)
+    before = _lib.lib().bb_kernel_launches()
+    got = quant_decode(q, kv, front=0, window=n, scale=d ** -0.5, n=n, splits=2)
+    assert _lib.lib().bb_kernel_launches() - before == 2
+    for i in (0, 77, 199):
+        want, spread, reach = qo.decode(f64(q[:, i:i + 1]), kval, vval, None, front=0, window=n, scale=d ** -0.5,
+                                        n=n - t + i + 1, weight=wval)
+        check_rounded(got[:, i:i + 1], want, spread, reach)
