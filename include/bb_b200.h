@@ -322,7 +322,8 @@ typedef struct {
 /* bb_qkv_write: rows k, v [Hkv, t, d] (fp16, bf16 or fp32; rows on 16-byte boundaries) into the cache
  * at positions at, at + 1, ... (at = *at_dev when at_dev != NULL); positions outside [0, cap) are
  * skipped. out_k / out_v (both or neither): the values that the written codes stand for, in the
- * input dtype, [Hkv, t, d] (also for skipped rows).
+ * input dtype, [Hkv, t, d] (also for skipped rows). As fp16, values beyond 65504 are infinite: the low value of a group
+ * that reaches below -65280 is -65536.
  *
  * bb_qkv_read: the values of rows start, start + 1, ... start + rows - 1, or of rows positions[Hkv, rows]
  * (int32, or int64 with pos_i64), as [Hkv, rows, d] in `dtype`; positions outside [0, cap) give zeros. */

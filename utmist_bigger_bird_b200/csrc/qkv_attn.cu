@@ -27,10 +27,11 @@
 // Scores, exponentials, sums and accumulators are fp32.
 //
 // What bounds it: bytes, 2 (d bits / 8 + 4 d / group) a key and KV head, and close behind them the issue slots that unpack
-// codes (about 580 warp instructions a step of 32 keys; HBM gives a SM a step every 220 cycles, so at 4 a cycle they
-// take 145). Measured on 8 KV heads x 4 query heads, d = 128, 4 bits, groups of 32: dense decode 36.5 us at 128K keys
-// (168 MB, 4.6 TB/s) and 51.7 us more for each 256K keys beyond (the rate of a copy); the rest, about 11 us, is the first
-// keys' latency and the merge of the splits.
+// codes (about 590 warp instructions a step of 32 keys; HBM gives a SM a step every 220 cycles, so at 4 a cycle they
+// take 150). Measured on 8 KV heads x 4 query heads, d = 128, 4 bits, groups of 32: dense decode 37.7 us at 128K keys
+// (168 MB, 4.5 TB/s) and 50 us more for each 256K keys beyond (the rate of a copy); the rest, about 12 us, is the first
+// keys' latency and the merge of the splits. More than 4 query rows of a KV head (several tokens) are bound by instructions:
+// every 8 rows unpack all codes anew, 89 us for 64 rows on 32K keys.
 #include <algorithm>
 #include <atomic>
 
@@ -595,7 +596,7 @@ template <bool SPLIT> struct Mask {
 // Warps a CTA and stages a warp: one CTA a SM (so that few partial results are left to merge), with 128 registers a
 // thread for 4 query rows in 4 bits, 168 for 8 rows and for 8 bits (whose stages are twice as large). Measured for 64
 // query rows on 32K keys (8 rows at a time): 12 warps 84.6 us, 10: 100, 14: 111, 16: 88; 16 rows at a time with 8 warps
-// of 255 registers: 95.
+// of 255 registers: 95 (all of them before each group had its own bound of the steps: 12 warps take 89 with it).
 template <int BITS, bool SPLIT> constexpr int warps() { return SPLIT && BITS == 4 ? 16 : 12; }
 constexpr int stages(int warps, int bytes) {
   const int fit = 225 * 1024 / (warps * bytes);
@@ -1142,7 +1143,7 @@ __device__ __forceinline__ void combine(const AttnParams& p, int64_t tile, int64
 // Grid (splits * ztiles, kv_heads). A warp owns its ring of stages and takes steps split * W + warp, then every
 // (splits * W)-th: no barrier until the warps' results are merged at the end. Adjacent warps take adjacent steps, so the
 // lists and ends, which come last, spread over the warps that have one step less to do. (Sparse step, 64 + 16384 + 512 of
-// 128K keys: 14.4 us; 8 query rows instead of 4 cost 20.0 instead of 16.2 us at 32K keys.)
+// 128K keys: 15.8 us; 8 query rows instead of 4 cost 21.0 instead of 16.9 us at 32K keys.)
 template <int BITS, int G, int NG, bool SPLIT>
 __global__ void __launch_bounds__(32 * warps<BITS, SPLIT>(), 1) qkv_partial_kernel(const AttnParams p) {
   using S = Stage<BITS, G, NG, true>;

@@ -275,7 +275,8 @@ def quant_decode(q, kv, indices=None, *, front=64, window=4096, scale=1.0, n=Non
     None for the whole capacity.
 
     Returns q's shape and dtype ([T, H, d] storage for T tokens). ``splits``: pieces that a key list is
-    cut into (default: enough to fill the GPU)."""
+    cut into (default: enough to fill the GPU). Any T up to 2^30 / H; every 8 query rows of a KV head
+    (H / Hkv a token) take a pass over the keys."""
     if q.ndim not in (2, 3):
         raise ValueError("quant_decode: q must be [H, d] or [H, T, d]")
     a, keep = _args(q, kv, front, window, scale, n, splits, "quant_decode")

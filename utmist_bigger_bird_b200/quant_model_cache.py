@@ -2,13 +2,14 @@
 cache, for models whose attention is ``RDAttention`` (``install``).
 
     install(model, "vs", sink=64, window=4096, vertical=512)
-    cache = make_quant_cache(model, capacity=131072, bits=4, sparse=dict(front=64, window=4096, k_route=512))
+    cache = make_quant_cache(model, capacity=131072, bits=4)
     logits = model(prompt_ids, past_key_values=cache).logits      # or model.generate(..., past_key_values=cache)
 
 ``update`` quantises the new rows. The first call of a layer (the prompt) returns the values that the rows now
 stand for, so the prefill attends to what later steps read; later calls return a handle whose ``attend``
 ``RDAttention.exact_attention`` calls: dense attention over the cache, or, for single tokens with ``sparse`` and a
-cache longer than front + window + k_route, ``quant_route`` and ``quant_decode`` over front | window | routes.
+cache longer than front + window + k_route, ``quant_route`` and ``quant_decode`` over front | window | routes (the
+routed result at a dense step's price or more: routing reads every key).
 Steps after the prompt require FP16 or BF16. ``RDAttention(kv_evict=True)`` works: the kept rows are quantised again in
 the place of the prompt.
 """
